@@ -52,6 +52,9 @@ extern "C" {
 #define WTQ_STATUS_LAYOUT 8        /* the scan kernel found its shared-memory plan unusable and did nothing */
 #define WTQ_STATUS_SCAN_TIMEOUT 16 /* a page copy of the scan kernel did not complete within its bounded wait */
 
+#define WTQ_STATUS_NO_PAGES 32     /* wtq_plan_tokens: too few free pages, or a table row too short; nothing was granted */
+#define WTQ_STATUS_BAD_PARENT 64   /* wtq_plan_tokens: a parent that does not stand before its child (taken as padding) */
+
 /* order of the fp32 summation in the rotation of wtq_quantize / wtq_append.
  * The reference computes (x/|x|) @ Pi^T with a CPU BLAS whose order depends
  * on the number of vectors in the call (turboquant_kv/cache.py:108-115);
@@ -271,6 +274,104 @@ int wtq_prefill(const void *q, int dtype, const int64_t q_strides[2], void *out,
                 float scale, int B, int Hq, int Hkv, int Q, int D, int S, int P, int max_pages,
                 int num_splits, void *workspace, size_t workspace_bytes, int32_t *status,
                 void *stream);
+
+/* ---- a speculative step: drafted trees, verified in one forward (no counterpart in the reference) ---- */
+
+/* Norms of queries and keys for each head with the rotary position rotation in one pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight   (weight NULL: no norm)
+ *   (a, b) -> (a cos - b sin, b cos + a sin)  over the first `rot` coordinates, pairs (i, i + rot / 2),
+ *                                             with `interleaved` (2 i, 2 i + 1)
+ * computed in fp32 and rounded once.  sides: q, k, v; heads = 0 leaves one out, v is only copied.
+ * x and out: element (b, head, token, d) at b * strides[0] + head * strides[1] + token * strides[2] + d;
+ * a side may be turned in place (out = x with the same strides) but must not overlap another way.
+ * positions (B, n), row stride in elements; table (table_rows, rot) fp32: the pairs' cosines, then
+ * their sines, row stride in elements.  weight (D) of `weight_dtype`.  A negative position is
+ * padding: that token's queries and keys become zeros; so they do at a position >= table_rows, which
+ * sets WTQ_STATUS_BAD_POSITION. */
+typedef struct {
+  const void *x;
+  void *out;
+  int64_t strides[3];      /* elements: batch, head, token */
+  int64_t out_strides[3];
+  const void *weight;
+  int heads;
+} wtq_rope_side_t;
+int wtq_qk_norm_rope(const wtq_rope_side_t sides[3], int dtype, int weight_dtype, float eps,
+                     const int32_t *positions, int64_t position_stride, const float *table,
+                     int64_t table_stride, int table_rows, int B, int n, int D, int rot, int interleaved,
+                     int32_t *status, void *stream);
+
+/* Block tables and slot maps of a step from request lengths.  Sequence b stores lengths[b] tokens, its
+ * row of `table` (B, max_pages) holds held[b] pages, and new_tokens[b] tokens are to follow.  Pages a
+ * sequence lacks come off the end of `free_pages` (the first *free_count of at most `stack` entries are
+ * free), in batch order, and their ids are written to the table.  `tokens` is the room of the per-token
+ * outputs; new tokens are numbered sequence by sequence.  With `parents` (B, drafted; row stride in
+ * elements) every sequence gets `drafted` tokens (new_tokens is not read): parent of a drafted token
+ * within its tree, -1 for one that follows the history's last token, -2 for padding; a parent stands
+ * before its child.  Outputs:
+ *   seq_lens, held (B), free_count (1)   the state after the step;
+ *   starts (B + 1)                       first token of each sequence, and their number;
+ *   sequence, positions (tokens)         of each token; in a tree the position is lengths[b] + depth,
+ *                                        -1 for padding;
+ *   slot_pages, slot_ends (tokens)       page and slot + 1 of each token, which always stands at place
+ *                                        lengths[b] + i: wtq_append takes them as page_table (max_pages
+ *                                        1) and seq_lens of single-token sequences;
+ *   mask (B, drafted, ceil(drafted/32))  with parents: bit j % 32 of word j / 32 is set where the token
+ *                                        sees tree token j (its ancestors and itself); 0 for padding.
+ * Entries past the last token read -1 (slot_ends 0).  A step that the free pages or the table's width do
+ * not cover is refused as a whole: no page is taken, seq_lens = lengths, every token entry is -1, the
+ * masks are 0, and WTQ_STATUS_NO_PAGES is set (WTQ_STATUS_BAD_POSITION for negative numbers or more new
+ * tokens than `tokens`).  State outputs may be the inputs; then `ticket`, a device word that is zero
+ * between calls, must be given.  B <= 4096. */
+typedef struct {
+  int32_t *seq_lens, *held, *free_count, *starts, *sequence, *positions, *slot_pages, *slot_ends, *mask;
+} wtq_plan_t;
+int wtq_plan_tokens(const int32_t *lengths, const int32_t *new_tokens, const int32_t *parents,
+                    int64_t parent_stride, int32_t *table, int64_t table_stride, const int32_t *held,
+                    const int32_t *free_pages, const int32_t *free_count, int B, int max_pages, int S,
+                    int tokens, int drafted, int stack, const wtq_plan_t *out, int32_t *ticket,
+                    int32_t *status, void *stream);
+/* The pages of the sequences with marks[b] != 0 go back onto the stack; their table rows read -1, their
+ * lengths and held counts 0.  More pages than `stack` has room for are refused (WTQ_STATUS_BAD_POSITION). */
+int wtq_release_tokens(const int32_t *marks, int32_t *table, int64_t table_stride, int32_t *lengths,
+                       int32_t *held, int32_t *free_pages, int32_t *free_count, int B, int max_pages,
+                       int stack, int32_t *status, void *stream);
+
+/* Attention of drafted trees over packed pages: the last Q tokens of every sequence (their K/V already
+ * appended, seq_lens includes them) each see the whole history before them and those of the Q tokens
+ * whose bit is set in their mask.  q, out: element (b, head, token, d) at b * strides[0] + head *
+ * strides[1] + token * strides[2] + d.  mask (B, Q, ceil(Q / 32)) int32 words, element strides {batch,
+ * token}; a token whose words are all zero is padding and gets zeros.  A sequence shorter than Q has no
+ * history, and tree tokens before its position 0 do not exist.  fp32 queries are computed in fp32 on the
+ * CUDA cores; 16-bit queries on the tensor cores (fp16 operands, fp32 sums) where head_dim is 64 or 128,
+ * the widths 4/4, 4/6, 6/6 or 8/8, the page size a power of two >= 16 and the pages 16-byte aligned,
+ * otherwise in fp32 as well.  head_dim <= 256, B <= 2048 x 65535.  Status bits as for wtq_decode.  The
+ * workspace (wtq_tree_workspace_bytes, 256-byte aligned) needs no preparation. */
+size_t wtq_tree_workspace_bytes(int B, int Hq, int Hkv, int Q, int D);
+int wtq_tree(const void *q, int dtype, const int64_t q_strides[3], void *out, const int64_t out_strides[3],
+             const wtq_side_t *k_side, const wtq_side_t *v_side, const int32_t *page_table,
+             int64_t table_stride, const int32_t *seq_lens, const int32_t *mask,
+             const int64_t mask_strides[2], float scale, int B, int Hq, int Hkv, int Q, int D, int S, int P,
+             int max_pages, void *workspace, size_t workspace_bytes, int32_t *status, void *stream);
+/* 1 where wtq_tree runs such a call on the tensor cores, 0 where in fp32. */
+int wtq_tree_on_tensor_cores(const wtq_side_t *k_side, const wtq_side_t *v_side, int dtype, int D, int S);
+
+/* The accepted tokens of a tree stay: of the last `drafted` tokens of sequence b, token keep[b][i] becomes
+ * token i for i < counts[b] (keep ascends; (B, most), row stride in elements), in every layer, as the
+ * codes and norms it has; out[b] = seq_lens[b] - drafted + counts[b].  out must not be seq_lens.  A path
+ * that does not ascend or leaves the tree keeps nothing of it (out[b] = seq_lens[b] - drafted; where that
+ * is negative, seq_lens[b]) and sets WTQ_STATUS_BAD_POSITION. */
+typedef struct {
+  uint8_t *pages;            /* all layers: (layers, P, Hkv, S, row_bytes) */
+  void *norms;               /* fp16 (layers, P, Hkv, S) */
+  int64_t layer_stride, page_stride, head_stride;                /* bytes */
+  int64_t norm_layer_stride, norm_page_stride, norm_head_stride; /* elements */
+  int row_bytes;
+} wtq_pool_side_t;
+int wtq_keep_tokens(const wtq_pool_side_t *k_side, const wtq_pool_side_t *v_side, const int32_t *page_table,
+                    int64_t table_stride, const int32_t *seq_lens, const int32_t *keep, int64_t keep_stride,
+                    const int32_t *counts, int layers, int B, int Hkv, int S, int P, int max_pages, int most,
+                    int drafted, int32_t *out, int32_t *status, void *stream);
 
 /* Replaces tq_dequant / tq_dequant_cuda (turboquant_kv/kernel.py:78-115,
  * turboquant_kv/csrc/tq_dequant.cu:186-211): N packed rows -> (N, D) of

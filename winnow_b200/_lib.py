@@ -14,6 +14,7 @@ WTQ_F32, WTQ_F16, WTQ_BF16 = 0, 1, 2
 ORDER_AUTO, ORDER_SEQUENTIAL, ORDER_INTERLEAVED16 = -1, 0, 1
 STATUS_BAD_PAGE, STATUS_BAD_POSITION = 1, 2
 STATUS_LAYOUT, STATUS_SCAN_TIMEOUT = 8, 16
+STATUS_NO_PAGES, STATUS_BAD_PARENT = 32, 64
 DEQUANT_AUTO, DEQUANT_EXACT, DEQUANT_TC, DEQUANT_TC_FAST = -1, 0, 1, 2
 DEQUANT_TC_MMA, DEQUANT_TC_FAST_MMA = 3, 4
 
@@ -38,6 +39,25 @@ class Exchange(ctypes.Structure):
     _fields_ = [("peer_out", c_void_p * 2), ("peer_flags", c_void_p),
                 ("out_strides", c_int64 * 2), ("rank", c_int), ("world", c_int),
                 ("head_offset", c_int), ("step_counter", c_void_p), ("done_counter", c_void_p)]
+
+
+class RopeSide(ctypes.Structure):
+    """Mirror of wtq_rope_side_t (include/winnow_tq.h)."""
+    _fields_ = [("x", c_void_p), ("out", c_void_p), ("strides", c_int64 * 3), ("out_strides", c_int64 * 3),
+                ("weight", c_void_p), ("heads", c_int)]
+
+
+class Plan(ctypes.Structure):
+    """Mirror of wtq_plan_t (include/winnow_tq.h)."""
+    _fields_ = [(name, c_void_p) for name in ("seq_lens", "held", "free_count", "starts", "sequence", "positions",
+                                              "slot_pages", "slot_ends", "mask")]
+
+
+class PoolSide(ctypes.Structure):
+    """Mirror of wtq_pool_side_t (include/winnow_tq.h)."""
+    _fields_ = [("pages", c_void_p), ("norms", c_void_p), ("layer_stride", c_int64), ("page_stride", c_int64),
+                ("head_stride", c_int64), ("norm_layer_stride", c_int64), ("norm_page_stride", c_int64),
+                ("norm_head_stride", c_int64), ("row_bytes", c_int)]
 
 
 STATUS_EXCHANGE_TIMEOUT = 4
@@ -100,6 +120,22 @@ _SIGNATURES = {
                             ctypes.POINTER(Side), ctypes.POINTER(Side), c_void_p, c_int64, c_void_p,
                             c_float, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                             c_void_p, c_size_t, c_void_p, c_void_p]),
+    "wtq_qk_norm_rope": (c_int, [ctypes.POINTER(RopeSide), c_int, c_int, c_float, c_void_p, c_int64, c_void_p,
+                                 c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "wtq_plan_tokens": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(Plan), c_void_p,
+                                c_void_p, c_void_p]),
+    "wtq_release_tokens": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                   c_int, c_void_p, c_void_p]),
+    "wtq_tree_workspace_bytes": (c_size_t, [c_int] * 5),
+    "wtq_tree": (c_int, [c_void_p, c_int, ctypes.POINTER(c_int64), c_void_p, ctypes.POINTER(c_int64),
+                         ctypes.POINTER(Side), ctypes.POINTER(Side), c_void_p, c_int64, c_void_p, c_void_p,
+                         ctypes.POINTER(c_int64), c_float, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                         c_void_p, c_size_t, c_void_p, c_void_p]),
+    "wtq_tree_on_tensor_cores": (c_int, [ctypes.POINTER(Side), ctypes.POINTER(Side), c_int, c_int, c_int]),
+    "wtq_keep_tokens": (c_int, [ctypes.POINTER(PoolSide), ctypes.POINTER(PoolSide), c_void_p, c_int64, c_void_p,
+                                c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                c_void_p, c_void_p, c_void_p]),
     "wtq_dequant": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                             c_int64, c_int64, c_int64, c_void_p]),
     "wtq_dequant_mode": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,

@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include "../../include/winnow_tq.h"
@@ -329,6 +330,275 @@ PyObject *stage(PyObject *, PyObject *const *a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+bool needs_grad(const at::Tensor &t) { return t.defined() && t.requires_grad() && c10::GradMode::is_enabled(); }
+bool optional(PyObject *o, at::Tensor &t) { return o == Py_None || tensor(o, t); }
+bool words(const at::Tensor &t, const at::Device &dev, at::IntArrayRef shape) {
+  return t.scalar_type() == at::kInt && t.device() == dev && t.sizes() == shape && t.is_contiguous();
+}
+PyObject *tuple_of(std::initializer_list<at::Tensor> ts) {
+  PyObject *r = PyTuple_New((Py_ssize_t)ts.size());
+  if (!r) return nullptr;
+  Py_ssize_t i = 0;
+  for (const at::Tensor &t : ts) {
+    PyObject *o = t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None);
+    if (!o) {
+      Py_DECREF(r);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(r, i++, o);
+  }
+  return r;
+}
+
+// rope(q, k, v, positions, table, q_weight, k_weight, eps, interleaved, out, status) -> (q, k[, v]), or None
+PyObject *rope(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  at::Tensor x[3], y[3], w[2], positions, table, status_tensor;
+  if (n != 11 || !tensor(a[0], x[0]) || !tensor(a[1], x[1]) || !optional(a[2], x[2]) || !tensor(a[3], positions) ||
+      !tensor(a[4], table) || !optional(a[5], w[0]) || !optional(a[6], w[1]) || !PyFloat_Check(a[7]))
+    Py_RETURN_NONE;
+  const int sides = x[2].defined() ? 3 : 2;
+  const at::Tensor &q = x[0];
+  const at::Device dev = q.device();
+  if (!q.is_cuda() || q.dim() != 4) Py_RETURN_NONE;
+  const int dtype = dtype_code(q.scalar_type());
+  const int64_t B = q.size(0), tokens = q.size(2), D = q.size(3);
+  int32_t *status;
+  if (dtype < 0 || B < 1 || tokens < 1 || D < 2 || !optional_status(a[10], dev, status_tensor, status)) Py_RETURN_NONE;
+  for (int i = 0; i < sides; ++i)
+    if (x[i].dim() != 4 || x[i].device() != dev || x[i].scalar_type() != q.scalar_type() || x[i].size(0) != B ||
+        x[i].size(1) < 1 || x[i].size(2) != tokens || x[i].size(3) != D || x[i].stride(3) != 1 || needs_grad(x[i]))
+      Py_RETURN_NONE;
+  if (sides == 3 && x[2].size(1) != x[1].size(1)) Py_RETURN_NONE;
+  int weight_dtype = dtype;
+  for (int i = 0; i < 2; ++i) {
+    if (!w[i].defined()) continue;
+    if (w[i].dim() != 1 || w[i].size(0) != D || !w[i].is_contiguous() || w[i].device() != dev || needs_grad(w[i]))
+      Py_RETURN_NONE;
+    weight_dtype = dtype_code(w[i].scalar_type());
+    if (weight_dtype < 0 || (w[0].defined() && w[i].scalar_type() != w[0].scalar_type())) Py_RETURN_NONE;
+  }
+  if (positions.dim() != 2 || positions.size(0) != B || positions.size(1) != tokens || positions.stride(1) != 1 ||
+      positions.scalar_type() != at::kInt || positions.device() != dev || table.dim() != 2 || table.stride(1) != 1 ||
+      table.scalar_type() != at::kFloat || table.device() != dev || table.size(1) > D || table.size(1) % 2)
+    Py_RETURN_NONE;
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  if (a[9] != Py_None) {                  // given outputs: buffers of their own, else the Python path looks closer
+    if (!PyTuple_Check(a[9]) || PyTuple_GET_SIZE(a[9]) != sides) Py_RETURN_NONE;
+    for (int i = 0; i < sides; ++i) {
+      if (!tensor(PyTuple_GET_ITEM(a[9], i), y[i]) || y[i].sizes() != x[i].sizes() || y[i].stride(3) != 1 ||
+          y[i].scalar_type() != q.scalar_type() || y[i].device() != dev || !y[i].is_contiguous())
+        Py_RETURN_NONE;
+      for (int j = 0; j < sides; ++j)
+        if (y[i].storage().data() == x[j].storage().data() || (j < i && y[i].storage().data() == y[j].storage().data()))
+          Py_RETURN_NONE;
+    }
+  } else {
+    for (int i = 0; i < sides; ++i) y[i] = at::empty(x[i].sizes(), q.options());
+  }
+  wtq_rope_side_t s[3] = {};
+  for (int i = 0; i < sides; ++i) {
+    s[i].x = x[i].const_data_ptr();
+    s[i].out = y[i].mutable_data_ptr();
+    for (int d = 0; d < 3; ++d) {
+      s[i].strides[d] = x[i].stride(d);
+      s[i].out_strides[d] = y[i].stride(d);
+    }
+    s[i].weight = i < 2 && w[i].defined() ? w[i].const_data_ptr() : nullptr;
+    s[i].heads = (int)x[i].size(1);
+  }
+  void *stream = (void *)at::cuda::getCurrentCUDAStream(dev.index()).stream();
+  const float eps = (float)PyFloat_AS_DOUBLE(a[7]);
+  const int turned = PyObject_IsTrue(a[8]) > 0;
+  int rc;
+  {
+    const Unlocked u;
+    rc = wtq_qk_norm_rope(s, dtype, weight_dtype, eps, positions.const_data_ptr<int32_t>(), positions.stride(0),
+                          table.const_data_ptr<float>(), table.stride(0), (int)table.size(0), (int)B, (int)tokens, (int)D,
+                          (int)table.size(1), turned, status, stream);
+  }
+  if (rc) return library_error(rc);
+  return sides == 3 ? tuple_of({y[0], y[1], y[2]}) : tuple_of({y[0], y[1]});
+  END_HANDLE_TH_ERRORS
+}
+
+// plan(lengths, new_tokens, table, held, free_pages, free_count, page_size, tokens, parents, out, ticket, status)
+// -> the nine tensors of a TokenPlan, or None
+PyObject *plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  at::Tensor lengths, fresh, table, held, free_pages, free_count, parents, ticket, status_tensor, o[9];
+  if (n != 12 || !tensor(a[0], lengths) || !optional(a[1], fresh) || !tensor(a[2], table) || !tensor(a[3], held) ||
+      !tensor(a[4], free_pages) || !tensor(a[5], free_count) || !PyLong_Check(a[6]) || !PyLong_Check(a[7]) ||
+      !optional(a[8], parents) || !optional(a[10], ticket))
+    Py_RETURN_NONE;
+  const int64_t S = PyLong_AsLongLong(a[6]), tokens = PyLong_AsLongLong(a[7]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  const at::Device dev = lengths.device();
+  int32_t *status;
+  if (!lengths.is_cuda() || table.dim() != 2 || table.scalar_type() != at::kInt || table.device() != dev ||
+      table.stride(1) != 1 || table.size(1) < 1 || S < 1 || S > INT32_MAX || tokens < 0 || tokens > INT32_MAX ||
+      !optional_status(a[11], dev, status_tensor, status))
+    Py_RETURN_NONE;
+  const int64_t B = table.size(0), W = table.size(1);
+  const int64_t Q = parents.defined() ? (parents.dim() == 2 ? parents.size(1) : 0) : 0, words_of = (Q + 31) / 32;
+  if (B < 1 || W > INT32_MAX || (B > 1 && table.stride(0) < W) || !words(lengths, dev, {B}) || !words(held, dev, {B}) ||
+      !words(free_count, dev, {1}) || free_pages.dim() != 1 || !words(free_pages, dev, {free_pages.size(0)}) ||
+      free_pages.size(0) > INT32_MAX || (ticket.defined() && !words(ticket, dev, {1})))
+    Py_RETURN_NONE;
+  if (parents.defined()) {
+    if (Q < 1 || parents.size(0) != B || parents.scalar_type() != at::kInt || parents.device() != dev ||
+        parents.stride(1) != 1 || B * Q != tokens || fresh.defined())
+      Py_RETURN_NONE;
+  } else if (!fresh.defined() || !words(fresh, dev, {B})) {
+    Py_RETURN_NONE;
+  }
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  if (a[9] != Py_None) {
+    if (!PyTuple_Check(a[9]) || PyTuple_GET_SIZE(a[9]) != 9 || !ticket.defined()) Py_RETURN_NONE;
+    for (int i = 0; i < 9; ++i)
+      if (!optional(PyTuple_GET_ITEM(a[9], i), o[i]) || (i < 8 && !o[i].defined())) Py_RETURN_NONE;
+    if (!words(o[0], dev, {B}) || !words(o[1], dev, {B}) || !words(o[2], dev, {1}) || !words(o[3], dev, {B + 1}) ||
+        !words(o[4], dev, {tokens}) || !words(o[5], dev, {tokens}) || !words(o[6], dev, {tokens, 1}) ||
+        !words(o[7], dev, {tokens}) || (parents.defined() && (!o[8].defined() || !words(o[8], dev, {B, Q, words_of}))))
+      Py_RETURN_NONE;
+  } else {
+    const auto opt = lengths.options();
+    o[0] = at::empty({B}, opt);
+    o[1] = at::empty({B}, opt);
+    o[2] = at::empty({1}, opt);
+    o[3] = at::empty({B + 1}, opt);
+    o[4] = at::empty({tokens}, opt);
+    o[5] = at::empty({tokens}, opt);
+    o[6] = at::empty({tokens, 1}, opt);
+    o[7] = at::empty({tokens}, opt);
+    if (parents.defined()) o[8] = at::empty({B, Q, words_of}, opt);
+  }
+  int32_t *p[9];
+  for (int i = 0; i < 9; ++i) p[i] = o[i].defined() ? o[i].mutable_data_ptr<int32_t>() : nullptr;
+  const wtq_plan_t out = {p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8]};
+  void *stream = (void *)at::cuda::getCurrentCUDAStream(dev.index()).stream();
+  int rc;
+  {
+    const Unlocked u;
+    rc = wtq_plan_tokens(lengths.const_data_ptr<int32_t>(), fresh.defined() ? fresh.const_data_ptr<int32_t>() : nullptr,
+                         parents.defined() ? parents.const_data_ptr<int32_t>() : nullptr,
+                         parents.defined() ? parents.stride(0) : 0, table.mutable_data_ptr<int32_t>(), table.stride(0),
+                         held.const_data_ptr<int32_t>(), free_pages.const_data_ptr<int32_t>(),
+                         free_count.const_data_ptr<int32_t>(), (int)B, (int)W, (int)S, (int)tokens, (int)Q,
+                         (int)free_pages.size(0), &out, ticket.defined() ? ticket.mutable_data_ptr<int32_t>() : nullptr,
+                         status, stream);
+  }
+  if (rc) return library_error(rc);
+  return tuple_of({o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7], o[8]});
+  END_HANDLE_TH_ERRORS
+}
+
+// tree(q, kv, mask, scale, out, workspace, status) -> out, or None
+PyObject *tree(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  at::Tensor q, mask, out, ws, status_tensor;
+  if (n != 7 || !tensor(a[0], q) || !tensor(a[2], mask) || !q.is_cuda() || q.dim() != 4 || q.stride(3) != 1)
+    Py_RETURN_NONE;
+  const int dtype = dtype_code(q.scalar_type());
+  const int64_t B = q.size(0), Hq = q.size(1), Q = q.size(2), D = q.size(3);
+  const at::Device dev = q.device();
+  Layer l;
+  int32_t *status;
+  if (dtype < 0 || B < 1 || Hq < 1 || Q < 1 || !read_layer(a[1], B, D, dev, l) || Hq % l.Hkv ||
+      !optional_status(a[6], dev, status_tensor, status))
+    Py_RETURN_NONE;
+  if (mask.dim() != 3 || mask.size(0) != B || mask.size(1) != Q || mask.size(2) != (Q + 31) / 32 ||
+      mask.stride(2) != 1 || mask.scalar_type() != at::kInt || mask.device() != dev)
+    Py_RETURN_NONE;
+  const double scale = PyFloat_AsDouble(a[3]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  if (a[4] != Py_None && (!tensor(a[4], out) || out.dim() != 4 || out.size(0) != B || out.size(1) != Hq ||
+                          out.size(2) != Q || out.size(3) != D || out.stride(3) != 1 ||
+                          out.scalar_type() != q.scalar_type() || out.device() != dev))
+    Py_RETURN_NONE;
+  if (a[5] != Py_None && (!tensor(a[5], ws) || ws.device() != dev || ws.scalar_type() != at::kByte || !ws.is_contiguous()))
+    Py_RETURN_NONE;
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  const bool fresh = !out.defined();
+  if (fresh) out = at::empty({B, Q, Hq, D}, q.options()).transpose(1, 2);
+  if (!ws.defined())
+    ws = at::empty({(int64_t)wtq_tree_workspace_bytes((int)B, (int)Hq, (int)l.Hkv, (int)Q, (int)D)},
+                   q.options().dtype(at::kByte));
+  const int64_t qs[3] = {q.stride(0), q.stride(1), q.stride(2)}, os[3] = {out.stride(0), out.stride(1), out.stride(2)};
+  const int64_t ms[2] = {mask.stride(0), mask.stride(1)};
+  void *stream = (void *)at::cuda::getCurrentCUDAStream(dev.index()).stream();
+  int rc;
+  {
+    const Unlocked u;
+    rc = wtq_tree(q.const_data_ptr(), dtype, qs, out.mutable_data_ptr(), os, &l.k, &l.v,
+                  l.table.const_data_ptr<int32_t>(), l.table.stride(0), l.lens.const_data_ptr<int32_t>(),
+                  mask.const_data_ptr<int32_t>(), ms, (float)scale, (int)B, (int)Hq, (int)l.Hkv, (int)Q, (int)D, (int)l.S,
+                  (int)l.P, (int)l.table.size(1), ws.mutable_data_ptr(), (size_t)ws.numel(), status, stream);
+  }
+  if (rc) return library_error(rc);
+  if (!fresh) return Py_NewRef(a[4]);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// keep(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, counts, drafted, out, status) -> lengths, or None
+PyObject *keep(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  at::Tensor pages[2], norms[2], table, lens, path, counts, out, status_tensor;
+  if (n != 11 || !tensor(a[0], pages[0]) || !tensor(a[1], norms[0]) || !tensor(a[2], pages[1]) || !tensor(a[3], norms[1]) ||
+      !tensor(a[4], table) || !tensor(a[5], lens) || !tensor(a[6], path) || !tensor(a[7], counts) || !PyLong_Check(a[8]) ||
+      !optional(a[9], out))
+    Py_RETURN_NONE;
+  const int64_t drafted = PyLong_AsLongLong(a[8]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  const at::Device dev = pages[0].device();
+  int32_t *status;
+  if (!pages[0].is_cuda() || drafted < 0 || drafted > INT32_MAX || table.dim() != 2 || table.scalar_type() != at::kInt ||
+      table.stride(1) != 1 || table.device() != dev || table.size(0) < 1 || table.size(1) < 1 ||
+      !optional_status(a[10], dev, status_tensor, status))
+    Py_RETURN_NONE;
+  const int64_t B = table.size(0);
+  wtq_pool_side_t s[2];
+  for (int i = 0; i < 2; ++i) {
+    const at::Tensor &p = pages[i], &m = norms[i];
+    if (p.dim() != 5 || m.dim() != 4 || p.device() != dev || m.device() != dev || p.scalar_type() != at::kByte ||
+        m.scalar_type() != at::kHalf || p.stride(4) != 1 || p.stride(3) != p.size(4) || m.stride(3) != 1 || p.numel() == 0)
+      Py_RETURN_NONE;
+    for (int d = 0; d < 4; ++d)
+      if (m.size(d) != p.size(d) || p.size(d) != pages[0].size(d)) Py_RETURN_NONE;
+    s[i] = {(uint8_t *)p.data_ptr(), m.data_ptr(), p.stride(0), p.stride(1), p.stride(2),
+            m.stride(0), m.stride(1), m.stride(2), (int)p.size(4)};
+  }
+  if (!words(lens, dev, {B}) || !words(counts, dev, {B}) || path.dim() != 2 || path.size(0) != B || path.size(1) < 1 ||
+      path.stride(1) != 1 || path.scalar_type() != at::kInt || path.device() != dev ||
+      (out.defined() && (!words(out, dev, {B}) || out.storage().data() == lens.storage().data())))
+    Py_RETURN_NONE;
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  if (!out.defined()) out = at::empty({B}, lens.options());
+  void *stream = (void *)at::cuda::getCurrentCUDAStream(dev.index()).stream();
+  int rc;
+  {
+    const Unlocked u;
+    rc = wtq_keep_tokens(&s[0], &s[1], table.const_data_ptr<int32_t>(), table.stride(0), lens.const_data_ptr<int32_t>(),
+                         path.const_data_ptr<int32_t>(), path.stride(0), counts.const_data_ptr<int32_t>(),
+                         (int)pages[0].size(0), (int)B, (int)pages[0].size(2), (int)pages[0].size(3),
+                         (int)pages[0].size(1), (int)table.size(1), (int)path.size(1), (int)drafted,
+                         out.mutable_data_ptr<int32_t>(), status, stream);
+  }
+  if (rc) return library_error(rc);
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject *set_error(PyObject *, PyObject *type) {
   Py_INCREF(type);
   Py_XSETREF(g_backend_error, type);
@@ -341,6 +611,13 @@ PyMethodDef methods[] = {
     {"append", (PyCFunction)(void (*)(void))append, METH_FASTCALL,
      "append(k, v, k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, k_tq, v_tq, order, status)"},
     {"stage", (PyCFunction)(void (*)(void))stage, METH_FASTCALL, "stage(dst, src, dst, src, dst, src)"},
+    {"rope", (PyCFunction)(void (*)(void))rope, METH_FASTCALL,
+     "rope(q, k, v, positions, table, q_weight, k_weight, eps, interleaved, out, status)"},
+    {"plan", (PyCFunction)(void (*)(void))plan, METH_FASTCALL,
+     "plan(lengths, new_tokens, table, held, free_pages, free_count, page_size, tokens, parents, out, ticket, status)"},
+    {"tree", (PyCFunction)(void (*)(void))tree, METH_FASTCALL, "tree(q, kv, mask, scale, out, workspace, status)"},
+    {"keep", (PyCFunction)(void (*)(void))keep, METH_FASTCALL,
+     "keep(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, counts, drafted, out, status)"},
     {"set_error", set_error, METH_O, "the exception type library errors are raised as"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "native host side of winnow_b200", -1, methods};

@@ -1,0 +1,160 @@
+// The accepted path of a drafted tree moves to the end of the kept history, in every layer: of the
+// `drafted` tokens a sequence appended, token keep[i] becomes token i (i = 0 .. count - 1), as the
+// codes and norms that it has, and the sequence ends there.  keep ascends, so keep[i] >= i.
+//
+// A warp takes the rows of one side of one (layer, sequence, kv head), sixteen-byte words of as
+// many rows as fit at a time: it reads them all, then writes them.  A batch of rows may only write
+// places up to its last row's, and every later source lies behind those, so the batches of a
+// warp can follow one another and no two warps meet.  Bound by the latency of three dependent
+// reads (path, table, row); 2 x the moved rows go over the bus.
+#include <algorithm>
+#include <type_traits>
+
+#include "wtq_common.cuh"
+
+namespace wtq {
+namespace keep {
+
+struct Side {
+  uint8_t *pages;
+  __half *norms;
+  int64_t layer_stride, page_stride, head_stride;                // bytes
+  int64_t norm_layer_stride, norm_page_stride, norm_head_stride; // elements
+  int nb;
+};
+struct Params {
+  Side side[2];
+  const int32_t *table, *seq_lens, *keep, *counts;
+  int64_t table_stride, keep_stride;
+  int B, Hkv, S, P, W, layers, A, drafted;
+  int32_t *out, *status;
+};
+
+constexpr int kThreads = 128;
+constexpr int kMost = 32;                 // rows looked up at a time
+
+// The path of a sequence holds: 0 <= keep[0] < keep[1] < .. < drafted, and the drafted tokens exist.
+__device__ __forceinline__ bool path_holds(const Params &p, int b, int lane, int &count, int &base) {
+  const int L = p.seq_lens[b];
+  count = p.counts[b];
+  base = L - p.drafted;
+  bool ok = base >= 0 && (int64_t)L <= (int64_t)p.W * p.S && count >= 0 && count <= p.A && count <= p.drafted;
+  for (int i = lane; ok && i < count; i += 32) {
+    const int k = p.keep[(int64_t)b * p.keep_stride + i];
+    const int up = i > 0 ? p.keep[(int64_t)b * p.keep_stride + i - 1] : -1;
+    ok = k > up && k < p.drafted && k >= 0;
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+
+// WORD bytes a lane: rows are multiples of it and aligned to it.
+template <int WORD>
+__global__ void __launch_bounds__(kThreads) keep_kernel(Params p) {
+  using T = typename std::conditional<WORD == 16, uint4, typename std::conditional<WORD == 4, uint32_t, uint8_t>::type>::type;
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  const int64_t units = (int64_t)p.layers * p.B * p.Hkv * 2;
+  if (unit >= units) return;
+  const int side = (int)(unit & 1);
+  const int h = (int)((unit >> 1) % p.Hkv);
+  const int b = (int)((unit >> 1) / p.Hkv % p.B);
+  const int layer = (int)((unit >> 1) / p.Hkv / p.B);
+  int count, base;
+  const bool ok = path_holds(p, b, lane, count, base);
+  if (layer == 0 && h == 0 && side == 0 && lane == 0) {
+    // (a malformed path: nothing is kept of the tree; a sequence too short for it stays as it is)
+    p.out[b] = ok ? base + count : base >= 0 ? base : p.seq_lens[b];
+    if (!ok && p.status) atomicOr(p.status, WTQ_STATUS_BAD_POSITION);
+  }
+  if (!ok) return;
+  const Side &sd = p.side[side];
+  const int words = sd.nb / WORD;                        // of a row
+  const int32_t *table = p.table + (int64_t)b * p.table_stride;
+  uint8_t *pages = sd.pages + layer * sd.layer_stride + h * sd.head_stride;
+  __half *norms = sd.norms + layer * sd.norm_layer_stride + h * sd.norm_head_stride;
+  for (int i0 = 0; i0 < count; i0 += kMost) {
+    const int rows = min(kMost, count - i0);
+    // lane r: where row i0 + r comes from and goes to (-1: it stays, or a page is not the pool's)
+    int64_t from = -1, to = -1;
+    __half norm = __ushort_as_half(0);
+    int64_t norm_to = -1;
+    if (lane < rows) {
+      const int i = i0 + lane, k = p.keep[(int64_t)b * p.keep_stride + i];
+      if (k != i) {
+        const int src = base + k, dst = base + i;
+        const int sp = table[src / p.S], dp = table[dst / p.S];
+        if ((uint32_t)sp < (uint32_t)p.P && (uint32_t)dp < (uint32_t)p.P) {
+          from = (int64_t)sp * sd.page_stride + (int64_t)(src % p.S) * sd.nb;
+          to = (int64_t)dp * sd.page_stride + (int64_t)(dst % p.S) * sd.nb;
+          norm = norms[(int64_t)sp * sd.norm_page_stride + src % p.S];
+          norm_to = (int64_t)dp * sd.norm_page_stride + dst % p.S;
+        } else if (p.status) {
+          atomicOr(p.status, WTQ_STATUS_BAD_PAGE);
+        }
+      }
+    }
+    __syncwarp();
+    if (norm_to >= 0) norms[norm_to] = norm;
+    // words of the rows in order, 32 x kIn at a time; row i's places lie at or before its source
+    constexpr int kIn = 4;
+    for (int w0 = 0; w0 < rows * words; w0 += 32 * kIn) {
+      T v[kIn];
+      int64_t dst[kIn];
+#pragma unroll
+      for (int j = 0; j < kIn; ++j) {
+        const int w = w0 + 32 * j + lane, r = min(w / words, kMost - 1);
+        const int64_t f = __shfl_sync(0xffffffffu, from, r), t = __shfl_sync(0xffffffffu, to, r);
+        dst[j] = w < rows * words && f >= 0 ? t + (int64_t)(w - r * words) * WORD : -1;
+        if (dst[j] >= 0) v[j] = *reinterpret_cast<const T *>(pages + f + (int64_t)(w - r * words) * WORD);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < kIn; ++j)
+        if (dst[j] >= 0) *reinterpret_cast<T *>(pages + dst[j]) = v[j];
+      __syncwarp();
+    }
+  }
+}
+
+}  // namespace keep
+}  // namespace wtq
+
+using namespace wtq;
+
+extern "C" int wtq_keep_tokens(const wtq_pool_side_t *k_side, const wtq_pool_side_t *v_side, const int32_t *page_table,
+                               int64_t table_stride, const int32_t *seq_lens, const int32_t *keep, int64_t keep_stride,
+                               const int32_t *counts, int layers, int B, int Hkv, int S, int P, int max_pages, int most,
+                               int drafted, int32_t *out, int32_t *status, void *stream_) {
+  if (!k_side || !v_side) return fail(WTQ_ERR_ARG, "wtq_keep_tokens: null sides");
+  if (layers < 1 || B < 0 || Hkv < 1 || S < 1 || P < 1 || max_pages < 1 || most < 0 || drafted < 0)
+    return fail(WTQ_ERR_ARG, "wtq_keep_tokens: bad sizes");
+  if (B == 0) return WTQ_OK;
+  if (!page_table || !seq_lens || !counts || !out || (most > 0 && !keep))
+    return fail(WTQ_ERR_ARG, "wtq_keep_tokens: null argument");
+  if (out == seq_lens) return fail(WTQ_ERR_ARG, "wtq_keep_tokens: out must not be seq_lens");
+  keep::Params p = {};
+  bool by16 = true, by4 = true;
+  const wtq_pool_side_t *sides[2] = {k_side, v_side};
+  for (int i = 0; i < 2; ++i) {
+    const wtq_pool_side_t &w = *sides[i];
+    if (!w.pages || !w.norms || w.row_bytes < 1) return fail(WTQ_ERR_ARG, "wtq_keep_tokens: null pages or norms");
+    p.side[i] = {w.pages, (__half *)w.norms, w.layer_stride, w.page_stride, w.head_stride, w.norm_layer_stride,
+                 w.norm_page_stride, w.norm_head_stride, w.row_bytes};
+    const uint64_t all = (uint64_t)(uintptr_t)w.pages | (uint64_t)w.layer_stride | (uint64_t)w.page_stride |
+                         (uint64_t)w.head_stride | (uint64_t)w.row_bytes;
+    by16 = by16 && all % 16 == 0;
+    by4 = by4 && all % 4 == 0;
+  }
+  p.table = page_table; p.seq_lens = seq_lens; p.keep = keep; p.counts = counts;
+  p.table_stride = table_stride; p.keep_stride = keep_stride;
+  p.B = B; p.Hkv = Hkv; p.S = S; p.P = P; p.W = max_pages; p.layers = layers; p.A = most; p.drafted = drafted;
+  p.out = out; p.status = status;
+  const int64_t units = (int64_t)layers * B * Hkv * 2, blocks = (units + 3) / 4;
+  if (blocks > 0x7fffffff) return fail(WTQ_ERR_ARG, "wtq_keep_tokens: too many rows");
+  cudaStream_t stream = (cudaStream_t)stream_;
+  if (by16) keep::keep_kernel<16><<<(unsigned)blocks, keep::kThreads, 0, stream>>>(p);
+  else if (by4) keep::keep_kernel<4><<<(unsigned)blocks, keep::kThreads, 0, stream>>>(p);
+  else keep::keep_kernel<1><<<(unsigned)blocks, keep::kThreads, 0, stream>>>(p);
+  note_launches(1);
+  return check_cuda(cudaGetLastError(), "wtq_keep_tokens launch");
+}

@@ -250,6 +250,78 @@ def prefill_supported(q: torch.Tensor, kv: pa.PackedKV) -> bool:
 
 
 @torch.no_grad()
+def tree_decode_attention(q: torch.Tensor, kv: pa.PackedKV, mask: torch.Tensor, scale: float, *,
+                          check_page_ids: bool = True, out: torch.Tensor | None = None,
+                          workspace: torch.Tensor | None = None,
+                          status: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of drafted trees over the packed pages (`wtq_tree`): q (B, Hq, Q, D) -> (B, Hq, Q, D) in
+    q.dtype, returned as a view of a (B, Q, Hq, D) tensor.
+
+    The Q drafted tokens of every sequence are appended already (`kv.seq_lens` includes them); each sees
+    the history before them and the tree tokens whose bit is set in its words of `mask`, int32
+    (B, Q, ceil(Q / 32)): bit j % 32 of word j // 32 (`plan_tokens` builds them from parents).  A token
+    without any bit is padding and gets zeros.  Any number of query heads per kv head, any width and
+    page size, head_dim up to 256.  fp32 queries are computed in fp32; 16-bit ones on the tensor cores
+    where the layout allows (`wtq_tree_on_tensor_cores`), and in fp32 elsewhere.  `workspace`: uint8, at
+    least `tree_workspace_bytes`, 256-byte aligned, needs no preparation; calls that may overlap need
+    one each."""
+    if not check_page_ids:                     # checked, allocated for and launched in native code
+        got = _lib.host().tree(q, kv, mask, scale, out, workspace, status)
+        if got is not None:
+            return got
+    pa.check_contract(q, kv, check_page_ids=check_page_ids)
+    if not q.is_cuda:
+        raise pa.UnsupportedLayout("the CUDA tree kernels need CUDA tensors")
+    B, Hq, Q, D = q.shape
+    dev = q.device
+    code = _lib.dtype_code(q.dtype)
+    if D > 256:
+        raise pa.UnsupportedLayout("head_dim above 256 is not supported")
+    for name, pages, norms in (("k", kv.k_pages, kv.k_norms), ("v", kv.v_pages, kv.v_norms)):
+        if pages.stride(-1) != 1 or pages.stride(-2) != pages.shape[-1] or norms.stride(-1) != 1:
+            raise pa.UnsupportedLayout(f"{name} pages need contiguous (S, NB) rows and contiguous norm slots")
+    for quant in (kv.k_quant, kv.v_quant):
+        if not quant.Pi.is_contiguous() or not quant.centroids.is_contiguous():
+            raise pa.UnsupportedLayout("rotations and codebooks must be contiguous")
+    if kv.page_table.stride(-1) != 1 or not kv.seq_lens.is_contiguous():
+        raise pa.UnsupportedLayout("page_table rows and seq_lens must be contiguous")
+    if tuple(mask.shape) != (B, Q, -(-Q // 32)) or mask.dtype != torch.int32 or mask.device != dev \
+            or (mask.shape[2] > 1 and mask.stride(2) != 1):
+        raise pa.UnsupportedLayout(f"mask must be int32 ({B}, {Q}, {-(-Q // 32)}) with contiguous words on {dev}")
+    if out is None:
+        out = torch.empty(B, Q, Hq, D, dtype=q.dtype, device=dev).permute(0, 2, 1, 3)
+    elif tuple(out.shape) != (B, Hq, Q, D) or out.dtype != q.dtype or out.device != dev or out.stride(-1) != 1:
+        raise pa.UnsupportedLayout("out must be (B, Hq, Q, D) in q.dtype with unit stride in D")
+    _lib.reachable("workspace", workspace)
+    _lib.reachable("status", status)
+    if B == 0 or Q == 0:
+        return out
+    Hkv, S, P = kv.num_kv_heads, kv.page_size, kv.k_pages.shape[0]
+    max_pages = kv.page_table.shape[1]
+    if max_pages == 0:
+        return out.zero_()
+    if q.stride(-1) != 1:
+        q = q.contiguous()
+    if workspace is None:
+        workspace = torch.empty(tree_workspace_bytes(B, Hq, Hkv, Q, D, dev), dtype=torch.uint8, device=dev)
+    k_side, v_side = _side(kv.k_pages, kv.k_norms, kv.k_quant), _side(kv.v_pages, kv.v_norms, kv.v_quant)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().wtq_tree(
+            q.data_ptr(), code, _lib.i64x(*q.stride()[:3]), out.data_ptr(), _lib.i64x(*out.stride()[:3]),
+            ctypes.byref(k_side), ctypes.byref(v_side), kv.page_table.data_ptr(), kv.page_table.stride(0),
+            kv.seq_lens.data_ptr(), mask.data_ptr(), _lib.i64x(*mask.stride()[:2]), float(scale), B, Hq, Hkv, Q, D, S,
+            P, max_pages, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+            status.data_ptr() if status is not None else None, _lib.stream_ptr(dev)))
+    return out
+
+
+def tree_workspace_bytes(B: int, Hq: int, Hkv: int, Q: int, D: int, device) -> int:
+    """Workspace of a `tree_decode_attention` call on `device`; it does not depend on the histories."""
+    with torch.cuda.device(device):
+        return _lib.lib().wtq_tree_workspace_bytes(B, Hq, Hkv, Q, D)
+
+
+@torch.no_grad()
 def dense_decode_attention(q: torch.Tensor, kv: "pa.DenseKV", scale: float, *, num_splits: int = 1,
                            allow_tf32: bool = False, num_warps: int = 4, num_stages: int = 2,
                            pages_per_iter: int = 1, status: torch.Tensor | None = None) -> torch.Tensor:

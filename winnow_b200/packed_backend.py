@@ -272,6 +272,66 @@ def append_tokens(k, v, k_pages, k_norms, v_pages, v_norms, page_table, seq_lens
             plan.run()
 
 
+def append_planned(k, v, k_pages, k_norms, v_pages, v_norms, plan, k_tq, v_tq, *,
+                   order: int = _lib.ORDER_AUTO, status: torch.Tensor | None = None) -> None:
+    """Fused append of a step's tokens to the slots of a `TokenPlan`, whatever number of them each
+    sequence has: k, v (T, Hkv, D) in the plan's order, row t to page slot_pages[t], slot
+    slot_ends[t] - 1.  The plan has exactly T tokens (a spare entry sets `STATUS_BAD_POSITION`)."""
+    if k.dim() != 3 or plan.slot_ends.shape != k.shape[:1]:
+        raise ValueError(f"k and v must be (T, Hkv, D) for the plan's {plan.slot_ends.numel()} tokens")
+    append_tokens(k.unsqueeze(2), v.unsqueeze(2), k_pages, k_norms, v_pages, v_norms, plan.slot_pages,
+                  plan.slot_ends, k_tq, v_tq, order=order, status=status)
+
+
+@torch.no_grad()
+def keep_tokens(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, counts, drafted: int, *,
+                out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """Keep a path of every sequence's last `drafted` tokens: token keep[b][i] becomes token i of them
+    for i < counts[b], in every layer, codes and norms as they are (`wtq_keep_tokens`); returns the
+    lengths after it, seq_lens - drafted + counts.
+
+    pages (layers, P, Hkv, S, NB) uint8, norms (layers, P, Hkv, S) fp16: a `PagePool`'s; page_table
+    (B, W), seq_lens (B,), counts (B,) and keep (B, A) int32, each row of keep ascending (what follows
+    its counts[b] entries is not read).  A row that does not ascend or leaves the tree keeps none of
+    its tokens and sets `STATUS_BAD_POSITION`.  `out` must not share memory with `seq_lens`."""
+    got = _lib.host().keep(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, counts, int(drafted), out,
+                           status)
+    if got is not None:
+        return got
+    dev = _lib.require_cuda(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, counts)
+    _lib.reachable("status", status)
+    if drafted < 0:
+        raise ValueError("drafted must not be negative")
+    if k_pages.dim() != 5 or v_pages.dim() != 5 or v_pages.shape[:4] != k_pages.shape[:4]:
+        raise ValueError("pages must be (layers, P, Hkv, S, NB)")
+    for pages, norms in ((k_pages, k_norms), (v_pages, v_norms)):
+        if pages.dtype != torch.uint8 or norms.dtype != torch.float16 or norms.shape != pages.shape[:4] \
+                or pages.stride(-1) != 1 or pages.stride(-2) != pages.shape[-1] or norms.stride(-1) != 1:
+            raise ValueError("pages need contiguous (S, NB) uint8 rows and norms contiguous fp16 slots")
+    B = page_table.shape[0]
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.stride(1) != 1:
+        raise ValueError("page_table must be int32 (B, W) with contiguous rows")
+    for name, t in (("seq_lens", seq_lens), ("counts", counts)) + ((("out", out),) if out is not None else ()):
+        if tuple(t.shape) != (B,) or t.dtype != torch.int32 or not t.is_contiguous() or t.device != dev:
+            raise ValueError(f"{name} must be contiguous int32 ({B},)")
+    if keep.dim() != 2 or keep.shape[0] != B or keep.dtype != torch.int32 or (keep.shape[1] > 1 and keep.stride(1) != 1):
+        raise ValueError("keep must be int32 (B, A) with contiguous rows")
+    if out is None:
+        out = torch.empty_like(seq_lens)
+    if B and out.data_ptr() == seq_lens.data_ptr():
+        raise ValueError("out must not share memory with seq_lens")
+    layers, P, Hkv, S, _ = k_pages.shape
+    sides = [_lib.PoolSide(pages.data_ptr(), norms.data_ptr(), *pages.stride()[:3], *norms.stride()[:3],
+                           pages.shape[4]) for pages, norms in ((k_pages, k_norms), (v_pages, v_norms))]
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().wtq_keep_tokens(
+            ctypes.byref(sides[0]), ctypes.byref(sides[1]), page_table.data_ptr(), page_table.stride(0),
+            seq_lens.data_ptr(), keep.data_ptr(), keep.stride(0), counts.data_ptr(), layers, B, Hkv, S, P,
+            page_table.shape[1], keep.shape[1], int(drafted), out.data_ptr(),
+            None if status is None else status.data_ptr(), _lib.stream_ptr(dev)))
+    return out
+
+
 def select_decode_backend(query: torch.Tensor, kv, requested: str) -> str:
     """Which operator serves a decode step.  Unsupported requests fail loudly."""
     if isinstance(kv, pa.DenseKV):
