@@ -4,20 +4,22 @@
 // The query rows of a group lie in tensor memory as the fp16 A operand of all score products.  The
 // group's tiles alternate between two streams, each with scores, probabilities, accumulator, running
 // maximum and sum of its own, so that one stream's softmax runs under the other's products; the two
-// states are joined when the piece ends.  Sixteen warps in three roles that meet at mbarriers only:
+// states are joined when the piece ends.  Sixteen warps in four roles that meet at mbarriers only:
 //
-//   decode    seven warps: tasks of 16 tokens of one side, codes loaded into registers two or three
-//             tasks ahead, through the per-lane lookup tables (wtq_lut.cuh) into the canonical operand
-//             layout, three tiles deep.  Keys go as centroids, their norms beside them in fp32 (the
-//             scores take them after the product, unrounded); values as centroid times norm;
+//   fetch     one warp: codes and norms of a tile as bulk copies into a ring of raw tiles, a lane per
+//             16 tokens of codes or norms of a side;
+//   decode    six warps: tasks of 16 tokens of one side through the per-lane lookup tables
+//             (wtq_lut.cuh) into the canonical operand layout, three tiles deep.  Keys go as
+//             centroids, their norms beside them in fp32 (the scores take them after the product,
+//             unrounded); values as centroid times norm;
 //   multiply  one warp, an elected lane issues: S = Q K^T (N 64) two tiles ahead of O += P V
 //             (A = P from tensor memory, V read with tokens as the contraction);
 //   softmax   a warpgroup per stream, a thread per query row: scores from tensor memory, handed back at
 //             once; norms, tree mask, running maximum, probabilities as fp16.  O is rescaled only when
 //             a row's maximum grows by 2^8.
 //
-// A piece's roles walk the static schedule by themselves: the decode warps work into the next piece
-// while the softmax warps write the last one's states.  Every wait is bounded; one that runs out
+// The roles walk the static schedule by themselves: fetch and decode work into the next piece while
+// the softmax warps write the last one's states.  Every wait is bounded; one that runs out
 // raises a flag that ends all others, and the status word says so.
 //
 // fp16 scores carry an error that grows with |q| |k|; a warp whose tile holds a row maximum beyond
@@ -36,7 +38,7 @@ namespace um {
 
 using namespace umma;
 
-constexpr int kSoftWarps = 8, kDecodeWarps = 7, kMmaWarp = kSoftWarps + kDecodeWarps;
+constexpr int kSoftWarps = 8, kDecodeWarps = 6, kFetchWarp = kSoftWarps + kDecodeWarps, kMmaWarp = kFetchWarp + 1;
 constexpr int kThreads = 32 * (kMmaWarp + 1);
 constexpr int kRows = kUmmaRows, kTile = kUmmaTile;
 constexpr int kStages = 3;                      // decoded tiles of a side
@@ -49,12 +51,15 @@ constexpr uint32_t kKFull = kBase, kVFull = kKFull + 8 * kStages, kKFree = kVFul
 constexpr uint32_t kSFull = kVFree + 8 * kStages, kSFree = kSFull + 16, kPFull = kSFree + 16,
                    kODone = kPFull + 16;                                   // [stream]
 constexpr uint32_t kNFull = kODone + 16;                                   // [ring]: key norms are there
-constexpr uint32_t kQFull = kNFull + 8 * kNormRing, kLast = kQFull + 8, kTmemSlot = kLast + 8, kAbort = kTmemSlot + 4;
+constexpr int kMostRaw = 5;                     // raw tiles: as many of these as fit
+constexpr uint32_t kRawFull = kNFull + 8 * kNormRing, kRawFree = kRawFull + 8 * kMostRaw;   // [raw tile]
+constexpr uint32_t kQFull = kRawFree + 8 * kMostRaw, kLast = kQFull + 8, kTmemSlot = kLast + 8, kAbort = kTmemSlot + 4;
+constexpr uint32_t kValid = kAbort + 4;                                    // [raw tile]: tokens of it that exist
 constexpr uint32_t kPrefix = kBase + 512;                                  // kMaxBatch + 1 words
 constexpr uint32_t kNorms = kPrefix + 4 * (kMaxBatch + 4);                 // [ring][64] fp32
 constexpr uint32_t kStates = kNorms + kNormRing * kTile * 4;               // [stream][m, l][row]
 constexpr uint32_t kVTile = 16384;
-static_assert(kAbort + 4 <= kPrefix && kStates + 4 * kRows * 4 <= kVTile, "low region");
+static_assert(kValid + 4 * kMostRaw <= kPrefix && kStates + 4 * kRows * 4 <= kVTile, "low region");
 static_assert(kVTile + kStages * kTile * 256 <= mma::kLutAddr, "value tiles end where the tables begin");
 // tensor memory columns
 constexpr uint32_t kColQ = 0, kColS = 64, kColP = 192, kColO = 256, kCols = 512;   // S + 64, P + 32, O + 128 per stream
@@ -68,11 +73,25 @@ template <int BWK, int BWV, int D> struct Map {
   static constexpr uint32_t kGroup = (uint32_t)D * 16u;                    // eight rows of an operand tile
   static constexpr uint32_t kTileBytes = kTile / 8 * kGroup;
   static constexpr uint32_t kKTile = mma::kLutAddr + (uint32_t)kEntries * 256u;
-  static constexpr uint32_t kDynamic = kKTile + kStages * kTileBytes;
-  static_assert(kDynamic <= 227u * 1024u, "shared memory budget");
+  // a raw tile: codes of K and V as the pages have them, then norms
+  static constexpr uint32_t kCodesK = kTile * D * BWK / 8, kCodesV = kTile * D * BWV / 8;
+  static constexpr uint32_t kRawBytes = kCodesK + kCodesV + 4 * kTile;
+  static constexpr uint32_t kRaw = kKTile + kStages * kTileBytes;
+  static constexpr int kFit = (int)((227u * 1024u - kRaw) / kRawBytes);
+  static constexpr int kRawTiles = kFit < kMostRaw ? kFit : kMostRaw;
+  static constexpr uint32_t kDynamic = kRaw + kRawTiles * kRawBytes;
+  static_assert(kRawTiles >= 2 && kDynamic <= 227u * 1024u, "shared memory budget");
   static constexpr uint32_t kIdescQK = (1u << 4) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
   static constexpr uint32_t kIdescPV = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
 };
+
+__device__ __forceinline__ void bulk_copy(uint32_t to, const void *from, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(to),
+               "l"(from), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void arrive_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
+}
 
 // Bounded wait for completion number `use` (0, 1, ..) of an mbarrier; false if it, or any
 // other wait of the block, ran out.
@@ -97,26 +116,7 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 }
 
 // ---- decode ------------------------------------------------------------------------------------
-// A lane's quarter of a packed row: D * BW / 32 bytes.
-template <int BW, int D> __device__ __forceinline__ void load_quarter(const uint8_t *at, uint32_t *w) {
-  constexpr int kBytes = D * BW / 32;
-  if constexpr (kBytes % 16 == 0) {
-#pragma unroll
-    for (int i = 0; i < kBytes / 16; ++i) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4 *>(at) + i);
-      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-    }
-  } else if constexpr (kBytes % 8 == 0) {
-#pragma unroll
-    for (int i = 0; i < kBytes / 8; ++i) {
-      const uint2 v = __ldg(reinterpret_cast<const uint2 *>(at) + i);
-      w[2 * i] = v.x; w[2 * i + 1] = v.y;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kBytes / 4; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t *>(at) + i);
-  }
-}
+// A lane's quarter of a packed row, D * BW / 32 bytes, is read by load_words of wtq_lut.cuh.
 // Codes 2 I, 2 I + 1 of the quarter as fp16 centroids.
 template <int BW, int I, int NW> __device__ __forceinline__ uint32_t two_codes(const uint32_t (&w)[NW], uint32_t sel) {
   if constexpr (BW == 4) return lut_byte<I % 4>(w[I / 4], sel);
@@ -254,6 +254,11 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(Params p) {
     }
 #pragma unroll
     for (int i = 0; i < kNormRing; ++i) mbar_init(kNFull + 8u * i, 4);
+#pragma unroll
+    for (int i = 0; i < kMostRaw; ++i) {
+      mbar_init(kRawFull + 8u * i, 1);
+      mbar_init(kRawFree + 8u * i, 8);                      // the eight tasks of a tile
+    }
     mbar_init(kQFull, kSoftWarps);
     mbar_init(kLast, 1);
     sts32(kAbort, 0u);
@@ -265,6 +270,11 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(Params p) {
   const uint32_t tmem = lds32(kTmemSlot);
   const long long share = run_length(p, prefix), all = (long long)prefix[p.B] * p.row_blocks * p.Hkv;
   const long long begin = share * blockIdx.x, end = min(all, begin + share);
+
+  // Registers go from the other warps to the softmax warps, which hold 64 scores a thread: 2 x 128 x
+  // (168 + 88) are the 512 x 128 that the block was launched with.
+  if (warp < kSoftWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;\n");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
 
   if (warp < kSoftWarps) {
     // ================= softmax: stream `st`, one query row per thread ====================
@@ -283,6 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(Params p) {
       const int i = qr / p.n_rep;
       const int32_t *words = p.mask + c.b * p.mask_b + i * p.mask_t;
       const bool live = qr < p.R && !padding(words, p.Q);
+      const bool working = __any_sync(kFull, live);         // a warp without live rows only keeps step
       const int64_t row = ((int64_t)c.b * p.Q + i) * p.Hq + c.h * p.n_rep + qr - i * p.n_rep;
       const float *q = live ? p.q_rot + row * D : nullptr;
       // this warpgroup's half of the query rows into tensor memory (the products of the last piece are done)
@@ -322,6 +333,15 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(Params p) {
         if (masked && live) {
           lo = visible(words, p.Q, tok0 - hist);
           hi = visible(words, p.Q, tok0 + 32 - hist);
+        }
+        if (!working) {
+          if (lane == 0) mbar_arrive(kSFree + 8u * st);
+          if (k > 0) {
+            ok = __all_sync(kFull, wait(kODone + 8u * st, n - 1));
+            if (!ok) break;
+          }
+          if (lane == 0) mbar_arrive(kPFull + 8u * st);
+          continue;
         }
         uint32_t s[64];
         tmem_load32<0>(s_addr, s);
@@ -427,113 +447,106 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(Params p) {
       tiles += nt;
       units += mine;
     }
-  } else if (warp < kMmaWarp) {
+  } else if (warp < kFetchWarp) {
     // ================= decode ==========================================================
-    // Tasks of 16 tokens of one side, eight per tile (four of K, four of V), dealt round-robin over
-    // all pieces; a cursor runs ahead, looking up pages, then loading codes.
-    constexpr int kWords = D * (BWK > BWV ? BWK : BWV) / 128;
-    constexpr int kAhead = kWords <= 4 ? 3 : 2;             // tasks whose codes are on their way
+    // Tasks of 16 tokens of one side, eight per tile (four of K, four of V), dealt round-robin.
     const int g = lane & 7, t = lane >> 3;
     const uint32_t sel = mma::kLutAddr | (uint32_t)(lane << 2);
-    struct Task {
-      int tile, q;                                          // tile of the run (-1: none); 0-3 K, 4-7 V
-      int tok, end, h, page;
-    };
-    long long x = begin;
-    Piece c = {};
-    int nt = 0, first_tile = 0, q = warp - kSoftWarps;      // q counts on from piece to piece
-    auto find_task = [&](Task &k) {                         // the cursor's task and its page id
-      while (q >= 8 * nt) {
-        q -= 8 * nt;
-        first_tile += nt;
-        if (x >= end) {
-          k.tile = -1;
-          nt = 0;
-          return;
-        }
-        c = piece_at(p, prefix, x, begin, end);
-        nt = c.last - c.first;
-        x += nt;
+    const long long tasks = 8 * max(0LL, end - begin);
+    auto task = [&](int T, int u, auto is_v_) -> bool {
+      constexpr bool kV = decltype(is_v_)::value;
+      constexpr int BW = kV ? BWV : BWK, kRowBytes = D * BW / 8;
+      const int raw = T % M::kRawTiles, buf = T % kStages;
+      if (!__all_sync(kFull, wait(kRawFull + 8u * raw, T / M::kRawTiles))) return false;
+      const uint32_t at = M::kRaw + (uint32_t)raw * M::kRawBytes, valid = lds32(kValid + 4u * raw);
+      const uint32_t codes = at + (kV ? M::kCodesK : 0u) + (uint32_t)(16 * u + g) * kRowBytes + (uint32_t)t * (kRowBytes / 4);
+      const uint32_t norms = at + M::kCodesK + M::kCodesV + (kV ? 2u * kTile : 0u) + (uint32_t)(16 * u + g) * 2u;
+      uint32_t w[2][kRowBytes / 16];
+      float n[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        load_words<kRowBytes / 4>(codes + (uint32_t)(8 * h) * kRowBytes, w[h]);
+        n[h] = (uint32_t)(16 * u + g + 8 * h) < valid ? lds_half(norms + 16u * h) : 0.f;
       }
-      k.tile = first_tile + (q >> 3);
-      k.q = q & 7;
-      k.tok = (c.first + (q >> 3)) * kTile + 16 * (q & 3);
-      k.end = length_of(p, c.b);
-      k.h = c.h;
-      k.page = k.tok < k.end ? p.page_table[(int64_t)c.b * p.table_stride + k.tok / p.S] : -2;
-      q += kDecodeWarps;
-    };
-    uint32_t w[kAhead][2][kWords];
-    __half nrm[kAhead][2];
-    int tile_of[kAhead], q_of[kAhead];
-    auto load = [&](const Task &k, uint32_t (&to)[2][kWords], __half (&n)[2]) {
-      const bool is_v = (k.q & 4) != 0;
-      const DecodeSideDev &sd = is_v ? p.v : p.k;
-      if ((uint32_t)k.page < (uint32_t)p.P) {
-        const int pos = k.tok & (p.S - 1);
-        const uint8_t *rows = sd.pages + (int64_t)k.page * sd.page_stride + (int64_t)k.h * sd.head_stride;
-        const __half *norms = sd.norms + (int64_t)k.page * sd.norm_page_stride + (int64_t)k.h * sd.norm_head_stride + pos;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = g + 8 * h;
-          if (BWK == BWV || !is_v) load_quarter<BWK, D>(rows + (int64_t)(pos + row) * (D * BWK / 8) + t * (D * BWK / 32), to[h]);
-          else load_quarter<BWV, D>(rows + (int64_t)(pos + row) * (D * BWV / 8) + t * (D * BWV / 32), to[h]);
-          n[h] = norms[row];
-          if (k.tok + row >= k.end) n[h] = __ushort_as_half(0);
-        }
-      } else {
-        if (k.page != -2 && p.status && lane == 0) atomicOr(p.status, WTQ_STATUS_BAD_PAGE);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int e = 0; e < kWords; ++e) to[h][e] = 0u;
-          n[h] = __ushort_as_half(0);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(kRawFree + 8u * raw);
+      if (T >= kStages)                                     // the tile's last reader is done
+        if (!__all_sync(kFull, wait((kV ? kVFree : kKFree) + 8u * buf, T / kStages - 1))) return false;
+      if constexpr (!kV) {
+        if (t == 0) {
+          const uint32_t to = kNorms + (uint32_t)(T % kNormRing) * (kTile * 4) + (uint32_t)(16 * u + g) * 4u;
+          sts32(to, __float_as_uint(n[0]));
+          sts32(to + 32, __float_as_uint(n[1]));
         }
       }
-    };
-    Task next;
-    find_task(next);
-#pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      tile_of[a] = next.tile;
-      q_of[a] = next.q;
-      if (next.tile >= 0) {
-        load(next, w[a], nrm[a]);
-        find_task(next);
+      const __half nh[2] = {__float2half_rn(n[0]), __float2half_rn(n[1])};
+      decode_task<BW, D, kV>((kV ? kVTile : M::kKTile) + (uint32_t)buf * M::kTileBytes, u, g, t, kV ? sel | 0x80u : sel, w, nh);
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive((kV ? kVFull : kKFull) + 8u * buf);
+        if (!kV) mbar_arrive(kNFull + 8u * (T % kNormRing));
       }
+      return true;
+    };
+    for (long long q = warp - kSoftWarps; q < tasks; q += kDecodeWarps) {
+      const int T = (int)(q >> 3), u = (int)q & 3;
+      if (!((q & 4) ? task(T, u, std::true_type{}) : task(T, u, std::false_type{}))) break;
     }
-    for (bool go = true; go;) {
-#pragma unroll
-      for (int a = 0; a < kAhead; ++a) {
-        const int T = tile_of[a], buf = T % kStages, u = q_of[a] & 3;
-        if (T < 0) { go = false; break; }
-        const bool is_v = (q_of[a] & 4) != 0;
-        if (T >= kStages) {                                 // the tile's last reader is done
-          const bool ok = wait((is_v ? kVFree : kKFree) + 8u * buf, T / kStages - 1);
-          if (!__all_sync(kFull, ok)) { go = false; break; }
+  } else if (warp == kFetchWarp) {
+    // ================= fetch ===========================================================
+    // lane: 16-token group lane & 3 of K codes, V codes, K norms, V norms (lane >> 2)
+    const int u = lane & 3, kind = lane >> 2;
+    const int page_shift = 31 - __clz(p.S);
+    const DecodeSideDev &sd = (kind & 1) ? p.v : p.k;
+    const uint32_t bytes = kind == 0 ? M::kCodesK / 4 : kind == 1 ? M::kCodesV / 4 : 2u * 16u;
+    const uint32_t to = (kind == 0 ? 0u : kind == 1 ? M::kCodesK : M::kCodesK + M::kCodesV + (kind == 3 ? 2u * kTile : 0u)) +
+                        (uint32_t)u * bytes;
+    int T = 0;
+    bool ok = true;
+    for (long long x = begin; x < end && ok;) {
+      const Piece c = piece_at(p, prefix, x, begin, end);
+      x += c.last - c.first;
+      const int L = length_of(p, c.b);
+      const int32_t *table = p.page_table + (int64_t)c.b * p.table_stride;
+      const uint8_t *codes = sd.pages + (int64_t)c.h * sd.head_stride;
+      const __half *norms = sd.norms + (int64_t)c.h * sd.norm_head_stride;
+      auto page_of = [&](int tile) {                        // -2: past the end
+        const int tok = tile * kTile + 16 * u;
+        return tile < c.last && tok < L ? table[tok >> page_shift] : -2;
+      };
+      int page = page_of(c.first), next = page_of(c.first + 1);
+      for (int tile = c.first; tile < c.last; ++tile, ++T) {
+        const int after = page_of(tile + 2);
+        const int raw = T % M::kRawTiles;
+        if (T >= M::kRawTiles) {
+          ok = __all_sync(kFull, wait(kRawFree + 8u * raw, T / M::kRawTiles - 1));
+          if (!ok) break;
         }
-        if (!is_v) {
-          if (t == 0) {
-            const uint32_t at = kNorms + (uint32_t)(T % kNormRing) * (kTile * 4) + (uint32_t)(16 * u + g) * 4u;
-            sts32(at, __float_as_uint(__half2float(nrm[a][0])));
-            sts32(at + 32, __float_as_uint(__half2float(nrm[a][1])));
+        const uint32_t at = M::kRaw + (uint32_t)raw * M::kRawBytes, bar = kRawFull + 8u * raw;
+        const bool good = (uint32_t)page < (uint32_t)p.P;
+        if (kind < 4 && !good) {
+          if (kind >= 2) {                                  // (codes of such tokens are whatever was there)
+            sts128(at + to, 0u, 0u, 0u, 0u);
+            sts128(at + to + 16, 0u, 0u, 0u, 0u);
+          } else if (kind == 0 && page != -2 && p.status) {
+            atomicOr(p.status, WTQ_STATUS_BAD_PAGE);
           }
-          decode_task<BWK, D, false>(M::kKTile + (uint32_t)buf * M::kTileBytes, u, g, t, sel, w[a], nrm[a]);
-        } else {
-          decode_task<BWV, D, true>(kVTile + (uint32_t)buf * M::kTileBytes, u, g, t, sel | 0x80u, w[a], nrm[a]);
         }
-        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-        __syncwarp();
+        const uint32_t fetched = __reduce_add_sync(kFull, kind < 4 && good ? bytes : 0u);
         if (lane == 0) {
-          mbar_arrive((is_v ? kVFull : kKFull) + 8u * buf);
-          if (!is_v) mbar_arrive(kNFull + 8u * (T % kNormRing));
+          sts32(kValid + 4u * raw, (uint32_t)min(kTile, L - tile * kTile));
+          arrive_expect(bar, fetched);
         }
-        tile_of[a] = next.tile;
-        q_of[a] = next.q;
-        if (next.tile >= 0) {
-          load(next, w[a], nrm[a]);
-          find_task(next);
+        __syncwarp();
+        if (kind < 4 && good) {
+          const int64_t slot = (tile * kTile + 16 * u) & (p.S - 1);
+          const void *from = kind < 2 ? (const void *)(codes + (int64_t)page * sd.page_stride + slot * (D / 8) * sd.bw)
+                                      : (const void *)(norms + (int64_t)page * sd.norm_page_stride + slot);
+          bulk_copy(at + to, from, bytes, bar);
         }
+        page = next;
+        next = after;
       }
     }
   } else {
@@ -635,7 +648,8 @@ template <int D> int launch_widths(const Params &p, cudaStream_t stream) {
 bool on_tensor_cores(const wtq_side_t &k, const wtq_side_t &v, int dtype, int D, int S) {
   const bool widths = (k.bw == 4 && (v.bw == 4 || v.bw == 6)) || (k.bw == v.bw && (k.bw == 6 || k.bw == 8));
   auto fits = [](const wtq_side_t &s) {
-    return ((uintptr_t)s.pages & 15) == 0 && s.page_stride % 16 == 0 && s.head_stride % 16 == 0;
+    return (((uintptr_t)s.pages | (uintptr_t)s.norms) & 15) == 0 && s.page_stride % 16 == 0 && s.head_stride % 16 == 0 &&
+           s.norm_page_stride % 8 == 0 && s.norm_head_stride % 8 == 0;
   };
   return dtype != WTQ_F32 && (D == 64 || D == 128) && widths && S >= 16 && (S & (S - 1)) == 0 && fits(k) && fits(v);
 }
