@@ -4,29 +4,31 @@
 // The query rows of a group lie in tensor memory as the fp16 A operand of all score products.  The
 // group's tiles alternate between two streams, each with scores, probabilities, accumulator, running
 // maximum and sum of its own, so that one stream's softmax runs under the other's products; the two
-// states are joined when the piece ends.  Sixteen warps in four roles that meet at mbarriers only:
+// states are joined when the piece ends.  Twenty-eight warps in roles that meet at mbarriers only:
 //
-//   fetch     one warp: codes and norms of a tile as bulk copies into a ring of raw tiles, a lane per
-//             16 tokens of codes or norms of a side;
-//   decode    six warps: tasks of 16 tokens of one side through the per-lane lookup tables
-//             (wtq_lut.cuh) into the canonical operand layout, three tiles deep.  Keys go as
-//             centroids, their norms beside them in fp32 (the scores take them after the product,
-//             unrounded); values as centroid times norm;
-//   multiply  one warp, an elected lane issues: S = Q K^T (N 64) two tiles ahead of O += P V
-//             (A = P from tensor memory, V read with tokens as the contraction);
-//   softmax   a warpgroup per stream, a thread per query row: scores from tensor memory, handed back at
-//             once; norms, tree mask, running maximum, probabilities as fp16.  O is rescaled only when
-//             a row's maximum grows by 2^8.
+//   fetch     a warp per side: codes and norms of a tile into a ring of raw tiles, 16 bytes a copy;
+//   decode    four warps per side, one for every 16 tokens of a tile: codes through the per-lane lookup
+//             tables (wtq_lut.cuh) to fp16 centroid times norm in the canonical operand layout, three
+//             tiles deep;
+//   multiply  a warp for S = Q K^T (N 64) and one for O += P V (A = P from tensor memory, V read with
+//             tokens as the contraction), an elected lane of each issues;
+//   softmax   two warpgroups per stream, a thread per query row and half of a tile's tokens: both take
+//             the maximum over the whole tile, which costs less than exchanging it, and the
+//             exponentials of their own half.  O is rescaled only when a row's maximum grows by 2^8.
 //
 // The roles walk the static schedule by themselves: fetch and decode work into the next piece while
-// the softmax warps write the last one's states.  Every wait is bounded; one that runs out
-// raises a flag that ends all others, and the status word says so.
+// the softmax warps write the last one's states.  Every wait is bounded; one that runs out raises a
+// flag that ends all others, and the status word says so.
+//
+// A warp on its own gets through an instruction in about nine cycles here, so a role is only as fast
+// as its instructions per tile are few: the split above gives every warp 100 to 150 of them.
 //
 // fp16 scores carry an error that grows with |q| |k|; a warp whose tile holds a row maximum beyond
 // kPreciseAbove (log2 domain) recomputes that tile's scores in fp32 from the packed codes.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
+#include <utility>
 
 #include "wtq_lut.cuh"
 #include "wtq_tree.cuh"
@@ -38,28 +40,24 @@ namespace um {
 
 using namespace umma;
 
-constexpr int kSoftWarps = 8, kDecodeWarps = 6, kFetchWarp = kSoftWarps + kDecodeWarps, kMmaWarp = kFetchWarp + 1;
-constexpr int kThreads = 32 * (kMmaWarp + 1);
+constexpr int kSoftWarps = 16, kDecodeWarp = kSoftWarps, kFetchWarp = kDecodeWarp + 8;
+constexpr int kScoreWarp = kFetchWarp + 2, kValueWarp = kScoreWarp + 1, kThreads = 32 * (kValueWarp + 1);
 constexpr int kRows = kUmmaRows, kTile = kUmmaTile;
 constexpr int kStages = 3;                      // decoded tiles of a side
-constexpr int kNormRing = 8;                    // tiles whose key norms are kept
+constexpr int kMostRaw = 5;                     // raw tiles of a side: as many of these as fit
 constexpr uint32_t kFull = 0xffffffffu;
 // shared memory; dynamic shared memory is assumed to start at or below kBase
 constexpr uint32_t kBase = 1024;
-constexpr uint32_t kKFull = kBase, kVFull = kKFull + 8 * kStages, kKFree = kVFull + 8 * kStages,
-                   kVFree = kKFree + 8 * kStages;                          // [stage]
-constexpr uint32_t kSFull = kVFree + 8 * kStages, kSFree = kSFull + 16, kPFull = kSFree + 16,
+constexpr uint32_t kTileFull = kBase, kTileFree = kTileFull + 16 * kStages;                 // [side][stage]
+constexpr uint32_t kRawFull = kTileFree + 16 * kStages, kRawFree = kRawFull + 16 * kMostRaw;   // [side][raw tile]
+constexpr uint32_t kSFull = kRawFree + 16 * kMostRaw, kSFree = kSFull + 16, kPFull = kSFree + 16,
                    kODone = kPFull + 16;                                   // [stream]
-constexpr uint32_t kNFull = kODone + 16;                                   // [ring]: key norms are there
-constexpr int kMostRaw = 5;                     // raw tiles: as many of these as fit
-constexpr uint32_t kRawFull = kNFull + 8 * kNormRing, kRawFree = kRawFull + 8 * kMostRaw;   // [raw tile]
-constexpr uint32_t kQFull = kRawFree + 8 * kMostRaw, kLast = kQFull + 8, kTmemSlot = kLast + 8, kAbort = kTmemSlot + 4;
-constexpr uint32_t kValid = kAbort + 4;                                    // [raw tile]: tokens of it that exist
+constexpr uint32_t kQFull = kODone + 16, kLast = kQFull + 8, kTmemSlot = kLast + 8, kAbort = kTmemSlot + 4;
+constexpr uint32_t kValid = kAbort + 4;                                    // [side][raw tile]: tokens of it that exist
 constexpr uint32_t kPrefix = kBase + 512;                                  // kMaxBatch + 1 words
-constexpr uint32_t kNorms = kPrefix + 4 * (kMaxBatch + 4);                 // [ring][64] fp32
-constexpr uint32_t kStates = kNorms + kNormRing * kTile * 4;               // [stream][m, l][row]
+constexpr uint32_t kStates = kPrefix + 4 * (kMaxBatch + 4);                // [stream][m, l of a half, l of the other][row]
 constexpr uint32_t kVTile = 16384;
-static_assert(kValid + 4 * kMostRaw <= kPrefix && kStates + 4 * kRows * 4 <= kVTile, "low region");
+static_assert(kValid + 8 * kMostRaw <= kPrefix && kStates + 6 * kRows * 4 <= kVTile, "low region");
 static_assert(kVTile + kStages * kTile * 256 <= mma::kLutAddr, "value tiles end where the tables begin");
 // tensor memory columns
 constexpr uint32_t kColQ = 0, kColS = 64, kColP = 192, kColO = 256, kCols = 512;   // S + 64, P + 32, O + 128 per stream
@@ -73,24 +71,20 @@ template <int BWK, int BWV, int D> struct Map {
   static constexpr uint32_t kGroup = (uint32_t)D * 16u;                    // eight rows of an operand tile
   static constexpr uint32_t kTileBytes = kTile / 8 * kGroup;
   static constexpr uint32_t kKTile = mma::kLutAddr + (uint32_t)kEntries * 256u;
-  // a raw tile: codes of K and V as the pages have them, then norms
-  static constexpr uint32_t kCodesK = kTile * D * BWK / 8, kCodesV = kTile * D * BWV / 8;
-  static constexpr uint32_t kRawBytes = kCodesK + kCodesV + 4 * kTile;
+  // a raw tile: codes as the pages have them, then norms
+  static constexpr uint32_t kRawK = kTile * D * BWK / 8 + 2 * kTile, kRawV = kTile * D * BWV / 8 + 2 * kTile;
   static constexpr uint32_t kRaw = kKTile + kStages * kTileBytes;
-  static constexpr int kFit = (int)((227u * 1024u - kRaw) / kRawBytes);
+  static constexpr int kFit = (int)((227u * 1024u - kRaw) / (kRawK + kRawV));
   static constexpr int kRawTiles = kFit < kMostRaw ? kFit : kMostRaw;
-  static constexpr uint32_t kDynamic = kRaw + kRawTiles * kRawBytes;
+  static constexpr uint32_t kDynamic = kRaw + kRawTiles * (kRawK + kRawV);
   static_assert(kRawTiles >= 2 && kDynamic <= 227u * 1024u, "shared memory budget");
   static constexpr uint32_t kIdescQK = (1u << 4) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
   static constexpr uint32_t kIdescPV = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
 };
 
-__device__ __forceinline__ void bulk_copy(uint32_t to, const void *from, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(to),
-               "l"(from), "r"(bytes), "r"(bar) : "memory");
-}
-__device__ __forceinline__ void arrive_expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
+// 16 bytes to shared memory, zeros where `there` is false (`from` is then not read).
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(from), "r"(there ? 16u : 0u) : "memory");
 }
 
 // Bounded wait for completion number `use` (0, 1, ..) of an mbarrier; false if it, or any
@@ -103,21 +97,26 @@ __device__ __forceinline__ bool wait(uint32_t bar, int use) {
   sts32(kAbort, 1u);
   return false;
 }
+__device__ __forceinline__ bool warp_wait(uint32_t bar, int use) { return __all_sync(kFull, wait(bar, use)); }
 
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
+// A place in a ring of N that is walked once: index and completion number without divisions.
+template <int N> struct Ring {
+  int at = 0, use = 0;
+  __device__ __forceinline__ void next() {
+    if (++at == N) {
+      at = 0;
+      ++use;
+    }
+  }
+};
+
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 
-// ---- decode ------------------------------------------------------------------------------------
-// A lane's quarter of a packed row, D * BW / 32 bytes, is read by load_words of wtq_lut.cuh.
-// Codes 2 I, 2 I + 1 of the quarter as fp16 centroids.
+// Codes 2 I, 2 I + 1 of a lane's quarter of a packed row as fp16 centroids.
 template <int BW, int I, int NW> __device__ __forceinline__ uint32_t two_codes(const uint32_t (&w)[NW], uint32_t sel) {
   if constexpr (BW == 4) return lut_byte<I % 4>(w[I / 4], sel);
   else return join(lut_code<BW, 2 * I>(w, sel), lut_code<BW, 2 * I + 1>(w, sel));
@@ -131,89 +130,165 @@ __device__ __forceinline__ uint32_t times(uint32_t c, __half2 n) {
   const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&c), n);
   return *reinterpret_cast<const uint32_t *>(&y);
 }
-// Rows g and g + 8 of tokens 16 u .. 16 u + 15, the quarter t of each, into an operand tile: all
-// lookups of a row go out before its stores.
-template <int BW, int D, bool SCALED, int NW>
-__device__ __forceinline__ void decode_task(uint32_t tile, int u, int g, int t, uint32_t sel, const uint32_t (&w)[2][NW],
-                                            const __half (&nrm)[2]) {
-  constexpr int kPairs = D / 8;                       // code pairs of a quarter
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t f[kPairs];
-    quarter_codes<BW>(w[h], sel, f, std::make_integer_sequence<int, kPairs>{});
-    if constexpr (SCALED) {
-      const __half2 n = __half2half2(nrm[h]);
-#pragma unroll
-      for (int i = 0; i < kPairs; ++i) f[i] = times(f[i], n);
-    }
-    const uint32_t at = tile + (uint32_t)(2 * u + h) * (uint32_t)(D * 16) + (uint32_t)t * (D / 32 * 128) + (uint32_t)g * 16u;
-#pragma unroll
-    for (int i = 0; i < kPairs / 4; ++i) sts128(at + 128u * i, f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
-  }
-}
 
-// fp32 products of this thread's query row with the 64 tokens' centroids, written over the tile's
-// scores in tensor memory: the packed codes are read from the pages (the same address for the whole
-// warp) and the row of `q` along with them.  Out of line: only for tiles whose scores came out large.
-template <int BW, int D>
-__device__ __noinline__ void precise_tile(const uint8_t *pages, int64_t page_stride, const float *centroids,
-                                          const int32_t *table, int P, int S, int tok0, int end, const float *q,
-                                          uint32_t s_addr) {
-  constexpr int kRowBytes = D * BW / 8;
-#pragma unroll 1
-  for (int blk = 0; blk < kTile / 16; ++blk) {                // sixteen tokens of one page
-    const int tok = tok0 + 16 * blk;
-    const int page = tok < end ? table[tok / S] : -1;
-    float acc[16];
+// One side's fetch warp: page ids of eight tiles ahead, a lane per 16 tokens.
+template <int BW, int D, int RAW_TILES>
+__device__ __forceinline__ void fetch_role(const Params &p, const DecodeSideDev &sd, const int *prefix, long long begin,
+                                           long long end, int side, uint32_t ring) {
+  constexpr int kBytes = 16 * D * BW / 8;                   // codes of 16 tokens
+  constexpr uint32_t kRawBytes = 4 * kBytes + 2 * kTile;
+  const int lane = threadIdx.x & 31, page_shift = 31 - __clz(p.S);
+  Ring<RAW_TILES> raw;
+  int T = 0;
+  for (long long x = begin; x < end;) {
+    const Piece c = piece_at(p, prefix, x, begin, end);
+    x += c.last - c.first;
+    const int L = length_of(p, c.b);
+    const int32_t *table = p.page_table + (int64_t)c.b * p.table_stride;
+    const uint8_t *codes = sd.pages + (int64_t)c.h * sd.head_stride;
+    const __half *norms = sd.norms + (int64_t)c.h * sd.norm_head_stride;
+    auto page_of = [&](int tile) {                          // of tokens 16 lane .. from that tile on; -2: past the end
+      const int tok = tile * kTile + 16 * lane;
+      return tok < L && tok < c.last * kTile ? table[tok >> page_shift] : -2;
+    };
+    int ahead = page_of(c.first);
+    uint32_t from_lo = 0, from_hi = 0;                      // where this lane's 16 tokens' codes are
+    const __half *norms_from = norms;
+    bool good = false;
+    for (int tile = c.first; tile < c.last; ++tile, ++T, raw.next()) {
+      const int step = (tile - c.first) & 7;
+      if (step == 0) {
+        const int page = ahead, slot = (tile * kTile + 16 * lane) & (p.S - 1);
+        ahead = page_of(tile + 8);
+        good = (uint32_t)page < (uint32_t)p.P;
+        if (!good && page != -2 && p.status) atomicOr(p.status, WTQ_STATUS_BAD_PAGE);
+        const uint64_t from = (uint64_t)(good ? codes + (int64_t)page * sd.page_stride + (int64_t)slot * (kBytes / 16) : codes);
+        from_lo = (uint32_t)from;
+        from_hi = (uint32_t)(from >> 32);
+        norms_from = good ? norms + (int64_t)page * sd.norm_page_stride + slot : norms;
+      }
+      const uint32_t bar = (uint32_t)(side * kMostRaw + raw.at) * 8u, at = ring + (uint32_t)raw.at * kRawBytes;
+      if (raw.use > 0 && !warp_wait(kRawFree + bar, raw.use - 1)) return;
+      const uint32_t goods = __ballot_sync(kFull, good) >> (4 * step);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-    if ((uint32_t)page < (uint32_t)P) {
-      const uint8_t *row = pages + (int64_t)page * page_stride + (int64_t)(tok % S) * kRowBytes;
-#pragma unroll 1
-      for (int d = 0; d < D / 4; ++d) {                        // four coordinates: BW / 2 bytes of each row
-        const float4 x = q ? __ldg(reinterpret_cast<const float4 *>(q) + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int u = 0; u < 4; ++u) {
+        const uint64_t lo = __shfl_sync(kFull, from_lo, 4 * step + u), hi = __shfl_sync(kFull, from_hi, 4 * step + u);
+        const uint8_t *from = (const uint8_t *)(lo | hi << 32);
+        const bool there = (goods >> u & 1u) != 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          uint32_t w = 0;
-#pragma unroll
-          for (int b = 0; b < BW / 2; ++b) w |= (uint32_t)__ldg(row + i * kRowBytes + d * (BW / 2) + b) << (8 * b);
-          constexpr uint32_t kMask = (1u << BW) - 1u;
-          acc[i] = fmaf(x.x, __ldg(centroids + (w & kMask)), acc[i]);
-          acc[i] = fmaf(x.y, __ldg(centroids + ((w >> BW) & kMask)), acc[i]);
-          acc[i] = fmaf(x.z, __ldg(centroids + ((w >> (2 * BW)) & kMask)), acc[i]);
-          acc[i] = fmaf(x.w, __ldg(centroids + ((w >> (3 * BW)) & kMask)), acc[i]);
-        }
+        for (int e = 0; e < kBytes; e += 512)
+          if (kBytes - e >= 512 || 16 * lane < kBytes - e)
+            copy16(at + (uint32_t)(u * kBytes + e) + 16u * lane, from + (there ? e + 16 * lane : 0), there);
+      }
+      if (lane >> 2 == step) {                              // the lane that knows the page
+        const uint32_t to = at + 4 * kBytes + 32u * (lane & 3);
+        copy16(to, norms_from, good);
+        copy16(to + 16, norms_from + (good ? 8 : 0), good);
+      }
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(kRawFull + bar) : "memory");
+      if (lane == 0) {
+        sts32(kValid + 4u * (uint32_t)(side * kMostRaw + raw.at), (uint32_t)min(kTile, L - tile * kTile));
+        mbar_arrive(kRawFull + bar);
       }
     }
-    uint32_t v[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(acc[i]);
-    __syncwarp();
-    tmem_store16(s_addr + 16 * blk, v);
   }
-  tmem_wait_store();
 }
 
-// Scores times key norms, those of unseen tokens -inf (`masked`: the tile reaches into the tree);
-// returns the row's maximum.
-__device__ __forceinline__ float norms_and_maximum(uint32_t (&s)[64], uint32_t norms, bool masked, uint32_t lo, uint32_t hi) {
+// One decode warp: tokens 16 u .. 16 u + 15 of every tile of a side, lane (g, t) rows g and g + 8,
+// coordinates t * D / 4 on.
+template <int BW, int D, int RAW_TILES>
+__device__ __forceinline__ void decode_role(int tiles, int side, int u, uint32_t ring, uint32_t tile_base) {
+  constexpr int kRowBytes = D * BW / 8, kPairs = D / 8;     // code pairs of a quarter
+  constexpr uint32_t kRawBytes = kTile * kRowBytes + 2 * kTile, kTileBytes = kTile * D * 2;
+  const int lane = threadIdx.x & 31, g = lane & 7, t = lane >> 3;
+  const uint32_t sel = mma::kLutAddr | (uint32_t)(lane << 2) | (side ? 0x80u : 0u);
+  const uint32_t row = (uint32_t)(16 * u + g);
+  const uint32_t codes = ring + row * kRowBytes + (uint32_t)t * (kRowBytes / 4), norms = ring + kTile * kRowBytes + 2u * row;
+  const uint32_t to = tile_base + (uint32_t)(2 * u) * (uint32_t)(D * 16) + (uint32_t)t * (D / 32 * 128) + (uint32_t)g * 16u;
+  const uint32_t raw_bar = kRawFull + (uint32_t)(side * kMostRaw) * 8u, tile_bar = kTileFull + (uint32_t)(side * kStages) * 8u;
+  constexpr uint32_t kFreeRaw = kRawFree - kRawFull, kFreeTile = kTileFree - kTileFull;
+  Ring<RAW_TILES> raw;
+  Ring<kStages> buf;
+  for (int T = 0; T < tiles; ++T, raw.next(), buf.next()) {
+    if (!warp_wait(raw_bar + 8u * raw.at, raw.use)) return;
+    // (looked at now, waited for only when the lookups are done)
+    const bool is_free = buf.use == 0 || mbar_try(tile_bar + kFreeTile + 8u * buf.at, (uint32_t)(buf.use - 1) & 1u);
+    const uint32_t off = (uint32_t)raw.at * kRawBytes;
+    const uint32_t valid = lds32(kValid + 4u * (uint32_t)(side * kMostRaw + raw.at));
+    uint32_t w[2][kRowBytes / 16];
+    __half2 n[2];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const uint4 n = lds128(norms + 16 * i);
-    const float2 a = halves(mul2(pair(__uint_as_float(s[4 * i]), __uint_as_float(s[4 * i + 1])),
-                                 pair(__uint_as_float(n.x), __uint_as_float(n.y))));
-    const float2 b = halves(mul2(pair(__uint_as_float(s[4 * i + 2]), __uint_as_float(s[4 * i + 3])),
-                                 pair(__uint_as_float(n.z), __uint_as_float(n.w))));
-    s[4 * i] = __float_as_uint(a.x); s[4 * i + 1] = __float_as_uint(a.y);
-    s[4 * i + 2] = __float_as_uint(b.x); s[4 * i + 3] = __float_as_uint(b.y);
-  }
-  if (masked) {
+    for (int h = 0; h < 2; ++h) {
+      load_words<kRowBytes / 4>(codes + off + (uint32_t)(8 * h * kRowBytes), w[h]);
+      n[h] = __float2half2_rn(row + 8u * h < valid ? lds_half(norms + off + 16u * h) : 0.f);
+    }
 #pragma unroll
-    for (int i = 0; i < 64; ++i) s[i] = ((i < 32 ? lo >> i : hi >> (i - 32)) & 1u) ? s[i] : 0xff800000u;
+    for (int h = 0; h < 2; ++h) {
+      uint32_t f[kPairs];
+      quarter_codes<BW>(w[h], sel, f, std::make_integer_sequence<int, kPairs>{});
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) f[i] = times(f[i], n[h]);
+      if (h == 0) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(raw_bar + kFreeRaw + 8u * raw.at);
+        if (!__all_sync(kFull, is_free) && !warp_wait(tile_bar + kFreeTile + 8u * buf.at, buf.use - 1)) return;
+      }
+      const uint32_t at = to + (uint32_t)buf.at * kTileBytes + (uint32_t)h * (uint32_t)(D * 16);
+#pragma unroll
+      for (int i = 0; i < kPairs / 4; ++i) sts128(at + 128u * i, f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+    }
+    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    __syncwarp();
+    if (lane == 0) mbar_arrive(tile_bar + 8u * buf.at);
   }
+}
+
+// fp32 scores of this thread's query row (null: zeros) with the sixteen tokens from `tok` on, from
+// the packed codes, the same address for the whole warp.  Out of line: only for tiles whose scores
+// came out large.
+template <int BW, int D>
+__device__ __noinline__ void precise_scores(const uint8_t *pages, int64_t page_stride, const __half *norms,
+                                            int64_t norm_page_stride, const float *centroids, const int32_t *table, int P,
+                                            int S, int tok, int end, const float *q, float *out) {
+  constexpr int kRowBytes = D * BW / 8;
+  const int page = tok < end ? table[tok / S] : -1;
+  float acc[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+  if ((uint32_t)page < (uint32_t)P) {
+    const uint8_t *row = pages + (int64_t)page * page_stride + (int64_t)(tok % S) * kRowBytes;
+#pragma unroll 1
+    for (int d = 0; d < D / 4; ++d) {                          // four coordinates: BW / 2 bytes of each row
+      const float4 x = q ? __ldg(reinterpret_cast<const float4 *>(q) + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int b = 0; b < BW / 2; ++b) w |= (uint32_t)__ldg(row + i * kRowBytes + d * (BW / 2) + b) << (8 * b);
+        constexpr uint32_t kMask = (1u << BW) - 1u;
+        acc[i] = fmaf(x.x, __ldg(centroids + (w & kMask)), acc[i]);
+        acc[i] = fmaf(x.y, __ldg(centroids + ((w >> BW) & kMask)), acc[i]);
+        acc[i] = fmaf(x.z, __ldg(centroids + ((w >> (2 * BW)) & kMask)), acc[i]);
+        acc[i] = fmaf(x.w, __ldg(centroids + ((w >> (3 * BW)) & kMask)), acc[i]);
+      }
+    }
+    const __half *nrm = norms + (int64_t)page * norm_page_stride + tok % S;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i] *= tok + i < end ? __half2float(nrm[i]) : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) out[i] = acc[i];
+}
+
+// Scores of unseen tokens become -inf (`seen`: a bit per token).
+__device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t seen) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) s[i] = (seen >> i & 1u) ? s[i] : 0xff800000u;
+}
+__device__ __forceinline__ float maximum(const uint32_t (&s)[32]) {
   float a = -INFINITY, c = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < 64; i += 4) {
+  for (int i = 0; i < 32; i += 4) {
     a = max3(a, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
     c = max3(c, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
   }
@@ -232,35 +307,31 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(Params p) {
   int *prefix = reinterpret_cast<int *>(dyn_smem + (kPrefix - (uint32_t)__cvta_generic_to_shared(dyn_smem)));
   for (int e = tid; e < M::kEntries * 64; e += kThreads)
     sts32(mma::kLutAddr + 4u * e, mma::lut_word(e, BWK, BWV, p.k.centroids, p.v.centroids));
-  if (warp == kMmaWarp) {
+  if (warp == kScoreWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(kTmemSlot),
                  "r"(kCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
   if (tid == 0) {
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(kKFull + 8u * i, 4);                        // the four 16-token groups of a tile
-      mbar_init(kVFull + 8u * i, 4);
-      mbar_init(kKFree + 8u * i, 1);
-      mbar_init(kVFree + 8u * i, 1);
+    for (int i = 0; i < 2 * kStages; ++i) {
+      mbar_init(kTileFull + 8u * i, 4);                     // the four 16-token groups of a tile
+      mbar_init(kTileFree + 8u * i, 1);
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * kMostRaw; ++i) {
+      mbar_init(kRawFull + 8u * i, 33);                     // 32 lanes' copies, and the word beside them
+      mbar_init(kRawFree + 8u * i, 4);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       mbar_init(kSFull + 8u * i, 1);
-      mbar_init(kSFree + 8u * i, 4);                        // the four warps of a stream
-      mbar_init(kPFull + 8u * i, 4);
+      mbar_init(kSFree + 8u * i, 8);                        // the eight warps of a stream
+      mbar_init(kPFull + 8u * i, 8);
       mbar_init(kODone + 8u * i, 1);
     }
-#pragma unroll
-    for (int i = 0; i < kNormRing; ++i) mbar_init(kNFull + 8u * i, 4);
-#pragma unroll
-    for (int i = 0; i < kMostRaw; ++i) {
-      mbar_init(kRawFull + 8u * i, 1);
-      mbar_init(kRawFree + 8u * i, 8);                      // the eight tasks of a tile
-    }
     mbar_init(kQFull, kSoftWarps);
-    mbar_init(kLast, 1);
+    mbar_init(kLast, 2);
     sts32(kAbort, 0u);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -271,50 +342,44 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(Params p) {
   const long long share = run_length(p, prefix), all = (long long)prefix[p.B] * p.row_blocks * p.Hkv;
   const long long begin = share * blockIdx.x, end = min(all, begin + share);
 
-  // Registers go from the other warps to the softmax warps, which hold 64 scores a thread: 2 x 128 x
-  // (168 + 88) are the 512 x 128 that the block was launched with.
-  if (warp < kSoftWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;\n");
-  else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
+  // Registers go from the other warps to the softmax warps: 512 x 88 + 384 x 48 of the 896 x 72 that
+  // the block was launched with.
+  if (warp < kSoftWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 88;\n");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");
 
   if (warp < kSoftWarps) {
-    // ================= softmax: stream `st`, one query row per thread ====================
-    const int st = warp >> 2, r = 32 * (warp & 3) + lane;
+    // ================= softmax: stream `st`, tokens 32 hf .. of its tiles, one query row per thread ======
+    const int st = warp >> 3, hf = (warp >> 2) & 1, r = 32 * (warp & 3) + lane;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t s_addr = tmem + lanes + kColS + 64u * st, p_addr = tmem + lanes + kColP + 32u * st,
+    const uint32_t s_addr = tmem + lanes + kColS + 64u * st, p_addr = tmem + lanes + kColP + 32u * st + 16u * hf,
                    o_addr = tmem + lanes + kColO + 128u * st;
-    int tiles = 0, units = 0;                               // tiles of the pieces before; units of this stream
+    int n = 0;                                              // units of this stream so far
     bool ok = true;
     for (long long x = begin; x < end;) {
       const Piece c = piece_at(p, prefix, x, begin, end);
       const int nt = c.last - c.first;
       x += nt;
       const int L = length_of(p, c.b), hist = L - p.Q, qr = c.rb * kRows + r;
-      const int32_t *table = p.page_table + (int64_t)c.b * p.table_stride;
       const int i = qr / p.n_rep;
       const int32_t *words = p.mask + c.b * p.mask_b + i * p.mask_t;
       const bool live = qr < p.R && !padding(words, p.Q);
       const bool working = __any_sync(kFull, live);         // a warp without live rows only keeps step
       const int64_t row = ((int64_t)c.b * p.Q + i) * p.Hq + c.h * p.n_rep + qr - i * p.n_rep;
       const float *q = live ? p.q_rot + row * D : nullptr;
-      // this warpgroup's half of the query rows into tensor memory (the products of the last piece are done)
-      if constexpr (D == 128) {
-        uint32_t v[32];
+      {
+        // this warpgroup's quarter of the query rows into tensor memory (the products of the last piece are done)
+        constexpr int kPart = D / 4;
+        const int part = warp >> 2;
+        uint32_t v[kPart / 2];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float4 y = q ? __ldg(reinterpret_cast<const float4 *>(q + 64 * st) + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < kPart / 4; ++k) {
+          const float4 y = q ? __ldg(reinterpret_cast<const float4 *>(q + kPart * part) + k) : make_float4(0.f, 0.f, 0.f, 0.f);
           v[2 * k] = pack_half2(y.x, y.y);
           v[2 * k + 1] = pack_half2(y.z, y.w);
         }
-        tmem_store32(tmem + lanes + kColQ + 32u * st, v);
-      } else {
-        uint32_t v[16];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float4 y = q ? __ldg(reinterpret_cast<const float4 *>(q + 32 * st) + k) : make_float4(0.f, 0.f, 0.f, 0.f);
-          v[2 * k] = pack_half2(y.x, y.y);
-          v[2 * k + 1] = pack_half2(y.z, y.w);
-        }
-        tmem_store16(tmem + lanes + kColQ + 16u * st, v);
+        const uint32_t to = tmem + lanes + kColQ + (uint32_t)(kPart / 2 * part);
+        if constexpr (D == 128) tmem_store16(to, v);
+        else tmem_store8(to, v);
       }
       tmem_wait_store();
       fence_before();
@@ -322,71 +387,81 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(Params p) {
       if (lane == 0) mbar_arrive(kQFull);
       float ref = -INFINITY, sum = 0.f;
       const int mine = (nt + 1 - st) / 2;                   // units of this stream in the piece
-      for (int k = 0; k < mine && ok; ++k) {
-        const int j = 2 * k + st, T = tiles + j, n = units + k, tok0 = (c.first + j) * kTile;
-        ok = wait(kSFull + 8u * st, n) && wait(kNFull + 8u * (T % kNormRing), T / kNormRing);
-        if (!__all_sync(kFull, ok)) { ok = false; break; }
-        fence_after();
-        const uint32_t norms = kNorms + (uint32_t)(T % kNormRing) * (kTile * 4);
-        const bool masked = tok0 + kTile > hist;
-        uint32_t lo = kFull, hi = kFull;
-        if (masked && live) {
-          lo = visible(words, p.Q, tok0 - hist);
-          hi = visible(words, p.Q, tok0 + 32 - hist);
-        }
+      for (int k = 0; k < mine && ok; ++k, ++n) {
+        const int tok0 = (c.first + 2 * k + st) * kTile;
+        if (!(ok = warp_wait(kSFull + 8u * st, n))) break;
         if (!working) {
           if (lane == 0) mbar_arrive(kSFree + 8u * st);
-          if (k > 0) {
-            ok = __all_sync(kFull, wait(kODone + 8u * st, n - 1));
-            if (!ok) break;
-          }
+          if (k > 0 && !(ok = warp_wait(kODone + 8u * st, n - 1))) break;
           if (lane == 0) mbar_arrive(kPFull + 8u * st);
           continue;
         }
-        uint32_t s[64];
-        tmem_load32<0>(s_addr, s);
-        tmem_load32<32>(s_addr + 32, s);
+        fence_after();
+        uint32_t s[32];
+        tmem_load32<0>(s_addr + 32u * (hf ^ 1), s);         // the other half, for its maximum
         tmem_wait_load();
-        float mx = norms_and_maximum(s, norms, masked, lo, hi);
-        if (__any_sync(kFull, !(fabsf(mx) <= kPreciseAbove) && mx != -INFINITY)) {
-          precise_tile<BWK, D>(p.k.pages + (int64_t)c.h * p.k.head_stride, p.k.page_stride, p.k.centroids, table, p.P,
-                               p.S, tok0, L, q, s_addr);
-          tmem_load32<0>(s_addr, s);
-          tmem_load32<32>(s_addr + 32, s);
-          tmem_wait_load();
-          mx = norms_and_maximum(s, norms, masked, lo, hi);
+        const bool masked = tok0 + kTile > hist;
+        uint32_t seen = kFull, seen_other = kFull;
+        if (masked && live) {
+          seen = visible(words, p.Q, tok0 + 32 * hf - hist);
+          seen_other = visible(words, p.Q, tok0 + 32 * (hf ^ 1) - hist);
         }
+        if (masked) hide(s, seen_other);
+        float mx = maximum(s);
+        tmem_load32<0>(s_addr + 32u * hf, s);
+        tmem_wait_load();
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(kSFree + 8u * st);       // the scores are in registers
-        if (k > 0) {                                        // the stream's last products have ended
-          ok = wait(kODone + 8u * st, n - 1);
-          if (!__all_sync(kFull, ok)) { ok = false; break; }
-          fence_after();
-        }
-        if (__any_sync(kFull, mx > ref + kSlack || (ref == -INFINITY && mx != -INFINITY))) {
+        if (masked) hide(s, seen);
+        mx = fmaxf(mx, maximum(s));
+        const bool large = !(fabsf(mx) <= kPreciseAbove) && mx != -INFINITY;
+        bool drained = k == 0;                              // the stream's last products have ended
+        if (__any_sync(kFull, large || mx > ref + kSlack || (ref == -INFINITY && mx != -INFINITY))) {
+          if (__any_sync(kFull, large)) {
+            const int32_t *table = p.page_table + (int64_t)c.b * p.table_stride;
+            float t16[16];
+            mx = -INFINITY;
+#pragma unroll
+            for (int blk = 0; blk < 4; ++blk) {             // the other half's tokens, then the own ones
+              const int half = blk < 2 ? hf ^ 1 : hf, tok = tok0 + 32 * half + 16 * (blk & 1);
+              precise_scores<BWK, D>(p.k.pages + (int64_t)c.h * p.k.head_stride, p.k.page_stride,
+                                     p.k.norms + (int64_t)c.h * p.k.norm_head_stride, p.k.norm_page_stride, p.k.centroids,
+                                     table, p.P, p.S, tok, L, q, t16);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const int bit = 16 * (blk & 1) + e;
+                const float v = ((blk < 2 ? seen_other : seen) >> bit & 1u) ? t16[e] : -INFINITY;
+                mx = fmaxf(mx, v);
+                if (blk >= 2) s[bit] = __float_as_uint(v);
+              }
+            }
+          }
           const float now = mx > ref + kSlack || ref == -INFINITY ? mx : ref;
-          if (k > 0) {                                      // rescale what is accumulated
+          if (k > 0 && __any_sync(kFull, now != ref)) {     // rescale what is accumulated
+            if (!(ok = warp_wait(kODone + 8u * st, n - 1))) break;
+            fence_after();
+            drained = true;
             const float scale = ref == now ? 1.f : ref == -INFINITY ? 0.f : ex2(ref - now);
             sum *= scale;
 #pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 32) {
-              uint32_t o[32];
-              tmem_load32<0>(o_addr + c0, o);
+            for (int c0 = hf * (D / 2); c0 < (hf + 1) * (D / 2); c0 += 16) {
+              uint32_t o[16];
+              tmem_load16(o_addr + c0, o);
               tmem_wait_load();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * scale);
-              tmem_store32(o_addr + c0, o);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * scale);
+              tmem_store16(o_addr + c0, o);
             }
             tmem_wait_store();
           }
           ref = now;
         }
         const uint64_t base = twice(ref == -INFINITY ? 0.f : -ref);
-        uint32_t pr[32];
+        uint32_t pr[16];
         uint64_t sums = 0;                                  // (the bits of two zeros)
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
+        for (int e = 0; e < 16; ++e) {
           const float2 y = halves(add2(pair(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), base));
           const float a = ex2(y.x), b = ex2(y.y);
           sums = add2(sums, pair(a, b));
@@ -394,226 +469,127 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(Params p) {
         }
         const float2 both = halves(sums);
         sum += both.x + both.y;
-        tmem_store32(p_addr, pr);
+        if (!drained) {                                     // the last products have read their probabilities
+          if (!(ok = warp_wait(kODone + 8u * st, n - 1))) break;
+          fence_after();
+        }
+        tmem_store16(p_addr, pr);
         tmem_wait_store();
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(kPFull + 8u * st);
       }
-      // ---- the rows' states: the two streams joined, half the coordinates to each warpgroup ----
-      if (ok && mine > 0) ok = wait(kODone + 8u * st, units + mine - 1);
-      ok = __all_sync(kFull, ok);
-      sts32(kStates + 4u * ((2 * st) * kRows + r), __float_as_uint(ref));
-      sts32(kStates + 4u * ((2 * st + 1) * kRows + r), __float_as_uint(sum));
+      // ---- the rows' states: the two streams joined, a quarter of the coordinates to each warpgroup ----
+      if (ok && mine > 0) ok = warp_wait(kODone + 8u * st, n - 1);
+      if (hf == 0) sts32(kStates + 4u * ((3 * st) * kRows + r), __float_as_uint(ref));
+      sts32(kStates + 4u * ((3 * st + 1 + hf) * kRows + r), __float_as_uint(sum));
       fence_before();
       asm volatile("bar.sync 1, %0;\n" ::"r"(32 * kSoftWarps) : "memory");   // every softmax warp, whatever it gave up on
       fence_after();
-      ok = ok && lds32(kAbort) == 0u;
-      ok = __all_sync(kFull, ok);
+      ok = __all_sync(kFull, ok && lds32(kAbort) == 0u);
       if (ok) {
-        const float m0 = __uint_as_float(lds32(kStates + 4u * r)), l0 = __uint_as_float(lds32(kStates + 4u * (kRows + r)));
-        const float m1 = __uint_as_float(lds32(kStates + 4u * (2 * kRows + r)));
-        const float l1 = __uint_as_float(lds32(kStates + 4u * (3 * kRows + r)));
-        const float top = fmaxf(m0, m1);
+        auto state = [&](int what) { return __uint_as_float(lds32(kStates + 4u * (what * kRows + r))); };
+        const float m0 = state(0), m1 = state(3), top = fmaxf(m0, m1);
         const float w0 = m0 == -INFINITY ? 0.f : ex2(m0 - top), w1 = m1 == -INFINITY ? 0.f : ex2(m1 - top);
+        const float total = w0 * (state(1) + state(2)) + w1 * (state(4) + state(5));
         float *acc;
         if (c.slot < 0) {
           acc = p.acc + row * D;
-          if (st == 0 && qr < p.R) p.m[row] = live ? top : -INFINITY, p.l[row] = live ? w0 * l0 + w1 * l1 : 0.f;
+          if (warp < 4 && qr < p.R) p.m[row] = live ? top : -INFINITY, p.l[row] = live ? total : 0.f;
         } else {
-          const int64_t s = ((int64_t)blockIdx.x * 2 + c.slot) * kRows + r;
-          acc = p.part_acc + s * D;
-          if (st == 0) p.part_m[s] = live ? top : -INFINITY, p.part_l[s] = live ? w0 * l0 + w1 * l1 : 0.f;
+          const int64_t at = ((int64_t)blockIdx.x * 2 + c.slot) * kRows + r;
+          acc = p.part_acc + at * D;
+          if (warp < 4) p.part_m[at] = live ? top : -INFINITY, p.part_l[at] = live ? total : 0.f;
         }
+        constexpr int kPart = D / 4;
+        const int part = warp >> 2;
 #pragma unroll 1
-        for (int c0 = st * (D / 2); c0 < (st + 1) * (D / 2); c0 += 32) {
-          uint32_t o[32], o1[32];
-          tmem_load32<0>(tmem + lanes + kColO + c0, o);
-          if (nt > 1) tmem_load32<0>(tmem + lanes + kColO + 128 + c0, o1);
+        for (int c0 = kPart * part; c0 < kPart * (part + 1); c0 += 16) {
+          uint32_t o[16], o1[16];
+          tmem_load16(tmem + lanes + kColO + c0, o);
+          if (nt > 1) tmem_load16(tmem + lanes + kColO + 128 + c0, o1);
           tmem_wait_load();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
+          for (int e = 0; e < 16; ++e) {
             float v = __uint_as_float(o[e]) * w0;
             if (nt > 1) v = fmaf(__uint_as_float(o1[e]), w1, v);
             o[e] = __float_as_uint(v);
           }
           if (live) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < 4; ++e)
               reinterpret_cast<uint4 *>(acc + c0)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
         }
       }
-      tiles += nt;
-      units += mine;
     }
   } else if (warp < kFetchWarp) {
-    // ================= decode ==========================================================
-    // Tasks of 16 tokens of one side, eight per tile (four of K, four of V), dealt round-robin.
-    const int g = lane & 7, t = lane >> 3;
-    const uint32_t sel = mma::kLutAddr | (uint32_t)(lane << 2);
-    const long long tasks = 8 * max(0LL, end - begin);
-    auto task = [&](int T, int u, auto is_v_) -> bool {
-      constexpr bool kV = decltype(is_v_)::value;
-      constexpr int BW = kV ? BWV : BWK, kRowBytes = D * BW / 8;
-      const int raw = T % M::kRawTiles, buf = T % kStages;
-      if (!__all_sync(kFull, wait(kRawFull + 8u * raw, T / M::kRawTiles))) return false;
-      const uint32_t at = M::kRaw + (uint32_t)raw * M::kRawBytes, valid = lds32(kValid + 4u * raw);
-      const uint32_t codes = at + (kV ? M::kCodesK : 0u) + (uint32_t)(16 * u + g) * kRowBytes + (uint32_t)t * (kRowBytes / 4);
-      const uint32_t norms = at + M::kCodesK + M::kCodesV + (kV ? 2u * kTile : 0u) + (uint32_t)(16 * u + g) * 2u;
-      uint32_t w[2][kRowBytes / 16];
-      float n[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        load_words<kRowBytes / 4>(codes + (uint32_t)(8 * h) * kRowBytes, w[h]);
-        n[h] = (uint32_t)(16 * u + g + 8 * h) < valid ? lds_half(norms + 16u * h) : 0.f;
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(kRawFree + 8u * raw);
-      if (T >= kStages)                                     // the tile's last reader is done
-        if (!__all_sync(kFull, wait((kV ? kVFree : kKFree) + 8u * buf, T / kStages - 1))) return false;
-      if constexpr (!kV) {
-        if (t == 0) {
-          const uint32_t to = kNorms + (uint32_t)(T % kNormRing) * (kTile * 4) + (uint32_t)(16 * u + g) * 4u;
-          sts32(to, __float_as_uint(n[0]));
-          sts32(to + 32, __float_as_uint(n[1]));
-        }
-      }
-      const __half nh[2] = {__float2half_rn(n[0]), __float2half_rn(n[1])};
-      decode_task<BW, D, kV>((kV ? kVTile : M::kKTile) + (uint32_t)buf * M::kTileBytes, u, g, t, kV ? sel | 0x80u : sel, w, nh);
-      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive((kV ? kVFull : kKFull) + 8u * buf);
-        if (!kV) mbar_arrive(kNFull + 8u * (T % kNormRing));
-      }
-      return true;
-    };
-    for (long long q = warp - kSoftWarps; q < tasks; q += kDecodeWarps) {
-      const int T = (int)(q >> 3), u = (int)q & 3;
-      if (!((q & 4) ? task(T, u, std::true_type{}) : task(T, u, std::false_type{}))) break;
-    }
-  } else if (warp == kFetchWarp) {
-    // ================= fetch ===========================================================
-    // lane: 16-token group lane & 3 of K codes, V codes, K norms, V norms (lane >> 2)
-    const int u = lane & 3, kind = lane >> 2;
-    const int page_shift = 31 - __clz(p.S);
-    const DecodeSideDev &sd = (kind & 1) ? p.v : p.k;
-    const uint32_t bytes = kind == 0 ? M::kCodesK / 4 : kind == 1 ? M::kCodesV / 4 : 2u * 16u;
-    const uint32_t to = (kind == 0 ? 0u : kind == 1 ? M::kCodesK : M::kCodesK + M::kCodesV + (kind == 3 ? 2u * kTile : 0u)) +
-                        (uint32_t)u * bytes;
-    int T = 0;
-    bool ok = true;
-    for (long long x = begin; x < end && ok;) {
-      const Piece c = piece_at(p, prefix, x, begin, end);
-      x += c.last - c.first;
-      const int L = length_of(p, c.b);
-      const int32_t *table = p.page_table + (int64_t)c.b * p.table_stride;
-      const uint8_t *codes = sd.pages + (int64_t)c.h * sd.head_stride;
-      const __half *norms = sd.norms + (int64_t)c.h * sd.norm_head_stride;
-      auto page_of = [&](int tile) {                        // -2: past the end
-        const int tok = tile * kTile + 16 * u;
-        return tile < c.last && tok < L ? table[tok >> page_shift] : -2;
-      };
-      int page = page_of(c.first), next = page_of(c.first + 1);
-      for (int tile = c.first; tile < c.last; ++tile, ++T) {
-        const int after = page_of(tile + 2);
-        const int raw = T % M::kRawTiles;
-        if (T >= M::kRawTiles) {
-          ok = __all_sync(kFull, wait(kRawFree + 8u * raw, T / M::kRawTiles - 1));
-          if (!ok) break;
-        }
-        const uint32_t at = M::kRaw + (uint32_t)raw * M::kRawBytes, bar = kRawFull + 8u * raw;
-        const bool good = (uint32_t)page < (uint32_t)p.P;
-        if (kind < 4 && !good) {
-          if (kind >= 2) {                                  // (codes of such tokens are whatever was there)
-            sts128(at + to, 0u, 0u, 0u, 0u);
-            sts128(at + to + 16, 0u, 0u, 0u, 0u);
-          } else if (kind == 0 && page != -2 && p.status) {
-            atomicOr(p.status, WTQ_STATUS_BAD_PAGE);
-          }
-        }
-        const uint32_t fetched = __reduce_add_sync(kFull, kind < 4 && good ? bytes : 0u);
-        if (lane == 0) {
-          sts32(kValid + 4u * raw, (uint32_t)min(kTile, L - tile * kTile));
-          arrive_expect(bar, fetched);
-        }
-        __syncwarp();
-        if (kind < 4 && good) {
-          const int64_t slot = (tile * kTile + 16 * u) & (p.S - 1);
-          const void *from = kind < 2 ? (const void *)(codes + (int64_t)page * sd.page_stride + slot * (D / 8) * sd.bw)
-                                      : (const void *)(norms + (int64_t)page * sd.norm_page_stride + slot);
-          bulk_copy(at + to, from, bytes, bar);
-        }
-        page = next;
-        next = after;
-      }
-    }
+    const int side = (warp - kDecodeWarp) >> 2, tiles = (int)max(0LL, end - begin);
+    if (side == 0) decode_role<BWK, D, M::kRawTiles>(tiles, 0, warp & 3, M::kRaw, M::kKTile);
+    else decode_role<BWV, D, M::kRawTiles>(tiles, 1, warp & 3, M::kRaw + M::kRawTiles * M::kRawK, kVTile);
+  } else if (warp < kScoreWarp) {
+    if (warp == kFetchWarp) fetch_role<BWK, D, M::kRawTiles>(p, p.k, prefix, begin, end, 0, M::kRaw);
+    else fetch_role<BWV, D, M::kRawTiles>(p, p.v, prefix, begin, end, 1, M::kRaw + M::kRawTiles * M::kRawK);
+    asm volatile("cp.async.wait_all;\n" ::: "memory");     // (a block that gave up leaves no copies behind)
   } else {
-    // ================= multiply: the whole warp waits, one lane issues ======================
+    // ================= multiply: one lane issues ===========================================
     const uint32_t issuer = elect_one();
-    int tiles = 0, pieces = 0, units[2] = {0, 0};
+    Ring<kStages> buf;
+    int pieces = 0, n0 = 0, n1 = 0;                         // units of the streams so far
     bool ok = true;
     for (long long x = begin; x < end && ok; ++pieces) {
       const Piece c = piece_at(p, prefix, x, begin, end);
       const int nt = c.last - c.first;
       x += nt;
-      ok = wait(kQFull, pieces);
-      if (!__all_sync(kFull, ok)) break;
-      fence_after();
-      auto scores = [&](int j) -> bool {                    // S of the piece's tile j
-        const int T = tiles + j, buf = T % kStages, st = j & 1, n = units[st] + (j >> 1);
-        if (!wait(kKFull + 8u * buf, T / kStages)) return false;
-        if (n > 0 && !wait(kSFree + 8u * st, n - 1)) return false;
+      if (warp == kScoreWarp) {
+        ok = warp_wait(kQFull, pieces);
         fence_after();
-        if (issuer) {
-          const uint64_t kb = descriptor(M::kKTile + (uint32_t)buf * M::kTileBytes, 128u, M::kGroup);
+        for (int j = 0; j < nt && ok; ++j, buf.next()) {    // S of the piece's tile j
+          const uint32_t st = j & 1;
+          const int n = st ? n1++ : n0++;
+          ok = __all_sync(kFull, (n == 0 || wait(kSFree + 8u * st, n - 1)) && wait(kTileFull + 8u * buf.at, buf.use));
+          fence_after();
+          if (ok && issuer) {
+            const uint64_t kb = descriptor(M::kKTile + (uint32_t)buf.at * M::kTileBytes, 128u, M::kGroup);
 #pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks)
-            umma_ts(tmem + kColS + 64u * st, tmem + kColQ + 8u * ks, kb + 16u * ks, M::kIdescQK, ks > 0);
-          umma_commit(kSFull + 8u * st);
-          umma_commit(kKFree + 8u * buf);
+            for (int ks = 0; ks < D / 16; ++ks)
+              umma_ts(tmem + kColS + 64u * st, tmem + kColQ + 8u * ks, kb + 16u * ks, M::kIdescQK, ks > 0);
+            umma_commit(kSFull + 8u * st);
+            umma_commit(kTileFree + 8u * buf.at);
+          }
+          __syncwarp();
         }
-        __syncwarp();
-        return true;
-      };
-      auto values = [&](int j) -> bool {                    // O += P V of tile j
-        const int T = tiles + j, buf = T % kStages, st = j & 1, n = units[st] + (j >> 1);
-        if (!wait(kVFull + 8u * buf, T / kStages)) return false;
-        if (!wait(kPFull + 8u * st, n)) return false;
-        fence_after();
-        if (issuer) {
-          const uint64_t vb = descriptor(kVTile + (uint32_t)buf * M::kTileBytes, M::kGroup, 128u);
+      } else {
+        for (int j = 0; j < nt && ok; ++j, buf.next()) {    // O += P V of tile j
+          const uint32_t st = j & 1, at = kStages + buf.at;
+          const int n = st ? n1++ : n0++;
+          ok = __all_sync(kFull, wait(kTileFull + 8u * at, buf.use) && wait(kPFull + 8u * st, n));
+          fence_after();
+          if (ok && issuer) {
+            const uint64_t vb = descriptor(kVTile + (uint32_t)buf.at * M::kTileBytes, M::kGroup, 128u);
 #pragma unroll
-          for (int ks = 0; ks < kTile / 16; ++ks)
-            umma_ts(tmem + kColO + 128u * st, tmem + kColP + 32u * st + 8u * ks, vb + (uint64_t)(2 * M::kGroup / 16) * ks,
-                    M::kIdescPV, j > 1 || ks > 0);
-          umma_commit(kODone + 8u * st);
-          umma_commit(kVFree + 8u * buf);
+            for (int ks = 0; ks < kTile / 16; ++ks)
+              umma_ts(tmem + kColO + 128u * st, tmem + kColP + 32u * st + 8u * ks, vb + (uint64_t)(2 * M::kGroup / 16) * ks,
+                      M::kIdescPV, j > 1 || ks > 0);
+            umma_commit(kODone + 8u * st);
+            umma_commit(kTileFree + 8u * at);
+          }
+          __syncwarp();
         }
-        __syncwarp();
-        return true;
-      };
-      for (int j = -2; j < nt && ok; ++j) {
-        if (j + 2 < nt) ok = scores(j + 2);
-        ok = __all_sync(kFull, ok);
-        if (ok && j >= 0) ok = values(j);
-        ok = __all_sync(kFull, ok);
       }
-      tiles += nt;
-      units[0] += (nt + 1) / 2;
-      units[1] += nt / 2;
     }
   }
   fence_before();
   __syncthreads();
   if (tid == 0 && lds32(kAbort) != 0u && p.status) atomicOr(p.status, WTQ_STATUS_SCAN_TIMEOUT);
-  if (warp == kMmaWarp) {
-    // A block that gave up may have products in flight: they end before their tensor memory
-    // goes to somebody else (bounded, like every wait).
+  // A block that gave up may have products in flight: they end before their tensor memory
+  // goes to somebody else (bounded, like every wait).  Each of the two warps answers for its own.
+  if (warp >= kScoreWarp) {
     fence_after();
     if (elect_one()) umma_commit(kLast);
     __syncwarp();
+  }
+  if (warp == kScoreWarp) {
     for (int spin = 0; spin < kWaitTries && !mbar_try(kLast, 0u); ++spin) {
     }
     __syncwarp();
