@@ -385,8 +385,8 @@ extern "C" int wtq_tree(const void *q, int dtype, const int64_t q_strides[3], vo
                                Hq, Hkv, D, S, P, max_pages))
     return rc;
   if (B == 0) return WTQ_OK;
-  if (B > 0 && (int64_t)B * Q > (int64_t)1 << 24)
-    return fail(WTQ_ERR_ARG, "wtq_tree: B * Q is limited to 2^24 query tokens");
+  if ((int64_t)B * Q > (int64_t)1 << 24 || (int64_t)B * Q * Hq > 0x7fffffff)
+    return fail(WTQ_ERR_ARG, "wtq_tree: B * Q is limited to 2^24 query tokens, B * Q * Hq to 2^31 rows");
   if ((int64_t)max_pages * S > (int64_t)1 << 30 ||
       (((int64_t)max_pages * S + 31) / 32) * std::min(B, tree::kMaxBatch) > 0x7fffffff)
     return fail(WTQ_ERR_ARG, "wtq_tree: the table covers too many tokens");
@@ -436,19 +436,30 @@ extern "C" int wtq_tree(const void *q, int dtype, const int64_t q_strides[3], vo
     p.part_l = take(parts * 4);
     const unsigned row_grid = (unsigned)((all + tree::kRowBlock - 1) / tree::kRowBlock);
     const size_t row_bytes = (size_t)tree::kRowBlock * (D + 4) * sizeof(float);
-    tree::rotate_kernel<<<row_grid, tree::kRowThreads, row_bytes, stream>>>(p);
-    note_launches(1);
-    if (int rc = check_cuda(cudaGetLastError(), "wtq_tree rotate launch")) return rc;
+    const bool products = tree::rows_on_tensor_cores(p);
     int rc;
+    if (products) {
+      rc = tree::launch_rotate(p, stream);
+    } else {
+      tree::rotate_kernel<<<row_grid, tree::kRowThreads, row_bytes, stream>>>(p);
+      note_launches(1);
+      rc = check_cuda(cudaGetLastError(), "wtq_tree rotate launch");
+    }
+    if (rc) return rc;
     if (umma) rc = tree::launch_scan_umma(p, stream);
     else if (D <= 64) rc = tree::launch_scan<1>(p, stream);
     else if (D <= 128) rc = tree::launch_scan<2>(p, stream);
     else if (D <= 192) rc = tree::launch_scan<3>(p, stream);
     else rc = tree::launch_scan<4>(p, stream);
     if (rc) return rc;
-    tree::join_kernel<<<row_grid, tree::kRowThreads, row_bytes, stream>>>(p);
-    note_launches(1);
-    if (int rc2 = check_cuda(cudaGetLastError(), "wtq_tree join launch")) return rc2;
+    if (products) {
+      rc = tree::launch_join(p, stream);
+    } else {
+      tree::join_kernel<<<row_grid, tree::kRowThreads, row_bytes, stream>>>(p);
+      note_launches(1);
+      rc = check_cuda(cudaGetLastError(), "wtq_tree join launch");
+    }
+    if (rc) return rc;
   }
   return WTQ_OK;
 }

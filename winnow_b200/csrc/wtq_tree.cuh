@@ -125,6 +125,9 @@ __device__ __forceinline__ bool padding(const int32_t *words, int Q) {
 
 bool on_tensor_cores(const wtq_side_t &k, const wtq_side_t &v, int dtype, int D, int S);
 int launch_scan_umma(const Params &p, cudaStream_t stream);
+bool rows_on_tensor_cores(const Params &p);
+int launch_rotate(const Params &p, cudaStream_t stream);
+int launch_join(const Params &p, cudaStream_t stream);
 constexpr int kUmmaRows = 128, kUmmaTile = 64;
 
 }  // namespace tree

@@ -1,0 +1,326 @@
+// The two products with a rotation either side of a tree scan, on the tensor cores, head_dim 64 or 128:
+// queries into the key basis (q_rot = q_scale * q Pi_K^T) and joined states out of the value basis
+// (out = a Pi_V, a = sum_c w_c acc_c / sum_c w_c l_c).
+//
+// 128 rows a block, one accumulator.  Both factors are split into fp16 high and low parts and three
+// products summed in fp32, which leaves 2^-22 of the result as error, the class of an fp32 product
+// (16-bit queries have no low part: two products).  A row is scaled by a power of two to its largest
+// element first, and Pi by 2^8, so that low parts stay clear of fp16's subnormal range.  Pi is laid out
+// as the operand once and serves both: read along its rows for the queries (K-major), across them for
+// the states (MN-major).  A thread per row quarter converts and stores.  Bound by the reads of rows and of
+// Pi from L2; at 16 384 rows the CUDA-core kernels of wtq_tree.cu took 187 and 70 us.
+#include <algorithm>
+#include <atomic>
+
+#include "wtq_tree.cuh"
+#include "wtq_umma.cuh"
+
+namespace wtq {
+namespace tree {
+namespace rows {
+
+using namespace umma;
+
+constexpr int kThreads = 512, kRows = 128;
+constexpr int kWaitTries = 1 << 20;
+constexpr float kPiScale = 256.f;
+
+template <int D> struct Map {
+  static constexpr uint32_t kGroup = (uint32_t)D * 16u;     // eight rows of an operand
+  static constexpr uint32_t kA = 1024, kABytes = kRows / 8 * kGroup;
+  static constexpr uint32_t kB = kA + 2 * kABytes, kBBytes = D / 8 * kGroup;
+  static constexpr uint32_t kScales = kB + 2 * kBBytes;     // a row's power of two
+  static constexpr uint32_t kBar = kScales + 4 * kRows, kSlot = kBar + 8, kPrefix = kSlot + 8;
+  static constexpr uint32_t kBytes = kPrefix + 4 * (kMaxBatch + 1);
+  static constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+};
+
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+// Eight values as fp16 high parts at `at`, what they leave as low parts at `at` + `low`.
+__device__ __forceinline__ void store_split(uint32_t at, uint32_t low, const float (&x)[8]) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    h[i] = half2_bits(x[2 * i], x[2 * i + 1]);
+    const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
+    l[i] = half2_bits(x[2 * i] - back.x, x[2 * i + 1] - back.y);
+  }
+  sts128(at, h[0], h[1], h[2], h[3]);
+  sts128(at + low, l[0], l[1], l[2], l[3]);
+}
+__device__ __forceinline__ void sts_float(uint32_t a, float v) {
+  asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(a), "f"(v) : "memory");
+}
+__device__ __forceinline__ float lds_float(uint32_t a) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(v) : "r"(a));
+  return v;
+}
+// The largest power of two not above |x|'s, and its inverse (1 for zeros and what is not finite).
+__device__ __forceinline__ float power_of(float x, float &inverse) {
+  const uint32_t e = __float_as_uint(x) >> 23 & 255u;
+  const bool plain = e >= 2 && e <= 252;
+  inverse = plain ? __uint_as_float((254u - e) << 23) : 1.f;
+  return plain ? __uint_as_float(e << 23) : 1.f;
+}
+
+__device__ __forceinline__ void place(const Params &p, int64_t row_, int &b, int &i, int &h) {
+  const uint32_t row = (uint32_t)row_, t = row / (uint32_t)p.Hq;       // (fewer than 2^31 rows)
+  h = (int)(row - t * (uint32_t)p.Hq);
+  b = (int)(t / (uint32_t)p.Q);
+  i = (int)(t - (uint32_t)b * (uint32_t)p.Q);
+}
+// x / share of tile numbers, in 32 bits where they fit
+__device__ __forceinline__ int run_of(long long x, long long share) {
+  return ((x | share) >> 31) == 0 ? (int)((uint32_t)x / (uint32_t)share) : (int)(x / share);
+}
+
+template <bool JOIN, int D>
+__global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms) {
+  using M = Map<D>;
+  extern __shared__ __align__(1024) uint8_t dyn_smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t base = (uint32_t)__cvta_generic_to_shared(dyn_smem);
+  if (base > 1024u) {
+    if (p.status && tid == 0) atomicOr(p.status, WTQ_STATUS_LAYOUT);
+    return;
+  }
+  constexpr int kPieces = D / 8;
+  const float *Pi = JOIN ? p.v.Pi : p.k.Pi;
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(M::kSlot), "r"((uint32_t)D)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  if (tid == 0) {
+    mbar_init(M::kBar, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+#pragma unroll
+  for (int e = tid; e < D * kPieces; e += kThreads) {
+    const int row = e / kPieces, piece = e % kPieces;
+    const float4 a = __ldg(reinterpret_cast<const float4 *>(Pi + row * D + 8 * piece));
+    const float4 b = __ldg(reinterpret_cast<const float4 *>(Pi + row * D + 8 * piece) + 1);
+    const float x[8] = {a.x * kPiScale, a.y * kPiScale, a.z * kPiScale, a.w * kPiScale,
+                        b.x * kPiScale, b.y * kPiScale, b.z * kPiScale, b.w * kPiScale};
+    store_split(M::kB + (uint32_t)(row >> 3) * M::kGroup + (uint32_t)piece * 128u + (uint32_t)(row & 7) * 16u, M::kBBytes, x);
+  }
+  int *prefix = reinterpret_cast<int *>(dyn_smem + (M::kPrefix - base));
+  long long share = 1;
+  if constexpr (JOIN) {
+    tile_prefix(p, prefix);
+    share = run_length(p, prefix);
+  }
+  // ---- the rows: kPieces lanes a row, several rows of a warp at a time ------------------------------
+  const int64_t rows = (int64_t)p.B * p.Q * p.Hq, row0 = (int64_t)blockIdx.x * kRows;
+  constexpr int kPerWarp = 32 / kPieces, kStep = kThreads / 32 * kPerWarp;
+  const int piece = lane % kPieces, first = warp * kPerWarp + lane / kPieces;
+  // all of a thread's loads of queries go out before the first is used
+  uint4 raw[JOIN ? 1 : kRows / kStep][2];
+  const bool wide = ((uintptr_t)p.q & 15) == 0 && (p.qb | p.qh | p.qt) % 8 == 0;
+  if constexpr (!JOIN) {
+#pragma unroll
+    for (int k = 0; k < kRows / kStep; ++k) {
+      const int64_t row = row0 + first + k * kStep;
+      raw[k][0] = raw[k][1] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < rows && wide) {
+        int b, i, h;
+        place(p, row, b, i, h);
+        const int64_t at = b * p.qb + i * p.qt + h * p.qh + 8 * piece;
+        const uint4 *from = reinterpret_cast<const uint4 *>((const char *)p.q + at * (p.dtype == WTQ_F32 ? 4 : 2));
+        raw[k][0] = __ldg(from);
+        if (p.dtype == WTQ_F32) raw[k][1] = __ldg(from + 1);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kRows / kStep; ++k) {
+    const int r = first + k * kStep;
+    const int64_t row = row0 + r;
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = 0.f;
+    int b = 0, i = 0, h = 0;
+    if (row < rows) place(p, row, b, i, h);
+    if constexpr (!JOIN) {
+      if (row < rows && !wide) {
+        const int64_t at = b * p.qb + i * p.qt + h * p.qh + 8 * piece;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = load_as_float(p.q, at + e, p.dtype);
+      } else {
+        const uint32_t w[8] = {raw[k][0].x, raw[k][0].y, raw[k][0].z, raw[k][0].w,
+                               raw[k][1].x, raw[k][1].y, raw[k][1].z, raw[k][1].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 v = p.dtype == WTQ_F16 ? __half22float2(*reinterpret_cast<const __half2 *>(&w[e]))
+                                              : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w[e]));
+          x[2 * e] = v.x;
+          x[2 * e + 1] = v.y;
+        }
+        if (p.dtype == WTQ_F32) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(w[e]);
+        }
+      }
+    } else {
+      const int n = row < rows ? prefix[b + 1] - prefix[b] : 0;
+      const int kvh = h / p.n_rep, qr = i * p.n_rep + h - kvh * p.n_rep, rb = qr / p.rows;
+      const long long g0 = (long long)prefix[b] * p.row_blocks * p.Hkv + (long long)(rb * p.Hkv + kvh) * n;
+      const int c0 = n > 0 ? run_of(g0, share) : 0, c1 = n > 0 ? run_of(g0 + n - 1, share) : -1;
+      auto add = [&](const float *acc, float w) {
+        const float4 a = __ldg(reinterpret_cast<const float4 *>(acc + 8 * piece));
+        const float4 c = __ldg(reinterpret_cast<const float4 *>(acc + 8 * piece) + 1);
+        x[0] = fmaf(w, a.x, x[0]); x[1] = fmaf(w, a.y, x[1]); x[2] = fmaf(w, a.z, x[2]); x[3] = fmaf(w, a.w, x[3]);
+        x[4] = fmaf(w, c.x, x[4]); x[5] = fmaf(w, c.y, x[5]); x[6] = fmaf(w, c.z, x[6]); x[7] = fmaf(w, c.w, x[7]);
+      };
+      if (c0 == c1) {                                       // an empty state's accumulator is not read
+        const float l = p.l[row];
+        if (l > 0.f) add(p.acc + row * D, 1.f / l);
+      } else if (c0 < c1) {
+        // the row's lanes look at a piece each; then all add up its coordinates, piece by piece
+        auto state = [&](int c) -> int64_t { return ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * p.rows + qr - rb * p.rows; };
+        const uint32_t group = (kPieces == 32 ? 0xffffffffu : ((1u << kPieces) - 1u)) << (lane / kPieces * kPieces);
+        float top = -INFINITY, sum = 0.f;
+        for (int c = c0 + piece; c <= c1; c += kPieces) top = fmaxf(top, p.part_m[state(c)]);
+#pragma unroll
+        for (int o = kPieces / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(group, top, o));
+        for (int from = c0; from <= c1; from += kPieces) {
+          const int c = from + piece;
+          const float m = c <= c1 ? p.part_m[state(c)] : -INFINITY;
+          const float w = m == -INFINITY ? 0.f : exp2f(m - top);
+          if (w > 0.f) sum = fmaf(w, p.part_l[state(c)], sum);
+          const int last = min(kPieces, c1 - from + 1);
+#pragma unroll 4
+          for (int e = 0; e < last; ++e) {
+            const float we = __shfl_sync(group, w, lane / kPieces * kPieces + e);
+            if (we > 0.f) add(p.part_acc + state(from + e) * D, we);
+          }
+        }
+#pragma unroll
+        for (int o = kPieces / 2; o; o >>= 1) sum += __shfl_xor_sync(group, sum, o);
+        const float f = sum > 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= f;
+      }
+    }
+    float most = 0.f, inverse;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[e]));
+#pragma unroll
+    for (int o = kPieces / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const float power = power_of(most, inverse);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= inverse;
+    store_split(M::kA + (uint32_t)(r >> 3) * M::kGroup + (uint32_t)piece * 128u + (uint32_t)(r & 7) * 16u, M::kABytes, x);
+    if (piece == 0) sts_float(M::kScales + 4u * r, power);
+  }
+  asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+  fence_before();
+  __syncthreads();
+  fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(tmem) : "r"(M::kSlot));
+  if (warp == 0) {
+    if (elect_one()) {
+      constexpr uint32_t kIdesc = M::kIdesc | (JOIN ? 1u << 16 : 0u);       // states: Pi is MN-major
+      for (int t = 0; t < terms; ++t) {                    // high x high, high x low, low x high
+        const uint64_t a = descriptor(M::kA + (t == 2 ? M::kABytes : 0u), 128u, M::kGroup);
+        const uint32_t from = M::kB + (t == 1 ? M::kBBytes : 0u);
+        const uint64_t b = JOIN ? descriptor(from, M::kGroup, 128u) : descriptor(from, 128u, M::kGroup);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks)
+          umma_ss(tmem, a + 16u * ks, b + (JOIN ? (uint64_t)(2 * M::kGroup / 16) * ks : 16u * ks), kIdesc, t > 0 || ks > 0);
+      }
+      umma_commit(M::kBar);
+    }
+    __syncwarp();
+  }
+  bool done = false;
+  for (int spin = 0; spin < kWaitTries && !done; ++spin) done = mbar_try(M::kBar, 0u);
+  if (!__syncthreads_and(done)) {
+    if (tid == 0 && p.status) atomicOr(p.status, WTQ_STATUS_SCAN_TIMEOUT);
+  }
+  fence_after();
+  // ---- a thread per row and quarter of the columns ---------------------------------------------------
+  const int r = 32 * (warp & 3) + lane;
+  const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+  const int64_t row = row0 + r;
+  const float f = lds_float(M::kScales + 4u * r) * (JOIN ? 1.f / kPiScale : p.q_scale / kPiScale);
+#pragma unroll 1
+  for (int c0 = (warp >> 2) * (D / 4); c0 < ((warp >> 2) + 1) * (D / 4); c0 += 16) {
+    uint32_t o[16];
+    tmem_load16(tmem + lanes + c0, o);
+    tmem_wait_load();
+    if (row >= rows || !done) continue;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+    if constexpr (!JOIN) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        reinterpret_cast<uint4 *>(p.q_rot + row * D + c0)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+    } else {
+      int b, i, h;
+      place(p, row, b, i, h);
+      const int64_t at = b * p.ob + i * p.ot + h * p.oh + c0;
+      char *dst = (char *)p.out + at * (p.dtype == WTQ_F32 ? 4 : 2);
+      if (((uintptr_t)dst & 15) != 0) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) store_from_float(p.out, at + e, __uint_as_float(o[e]), p.dtype);
+      } else if (p.dtype == WTQ_F32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          reinterpret_cast<uint4 *>(dst)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+      } else {
+        uint32_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = __uint_as_float(o[2 * e]), y = __uint_as_float(o[2 * e + 1]);
+          const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+          w[e] = p.dtype == WTQ_F16 ? half2_bits(x, y) : *reinterpret_cast<const uint32_t *>(&v);
+        }
+        reinterpret_cast<uint4 *>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint4 *>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+      }
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"((uint32_t)D) : "memory");
+}
+
+template <bool JOIN, int D> int launch(const Params &p, cudaStream_t stream) {
+  using M = Map<D>;
+  static std::atomic<bool> opted_in[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !opted_in[dev & 63].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(product_kernel<JOIN, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)M::kBytes);
+    if (e != cudaSuccess) return check_cuda(e, "wtq_tree: shared memory opt-in");
+    opted_in[dev & 63].store(true, std::memory_order_release);
+  }
+  const int64_t all = (int64_t)p.B * p.Q * p.Hq;
+  product_kernel<JOIN, D><<<(unsigned)((all + kRows - 1) / kRows), kThreads, M::kBytes, stream>>>(
+      p, JOIN || p.dtype == WTQ_F32 ? 3 : 2);
+  note_launches(1);
+  return check_cuda(cudaGetLastError(), "wtq_tree product launch");
+}
+
+}  // namespace rows
+
+bool rows_on_tensor_cores(const Params &p) {
+  return (p.D == 64 || p.D == 128) && (((uintptr_t)p.k.Pi | (uintptr_t)p.v.Pi) & 15) == 0;
+}
+int launch_rotate(const Params &p, cudaStream_t stream) {
+  return p.D == 128 ? rows::launch<false, 128>(p, stream) : rows::launch<false, 64>(p, stream);
+}
+int launch_join(const Params &p, cudaStream_t stream) {
+  return p.D == 128 ? rows::launch<true, 128>(p, stream) : rows::launch<true, 64>(p, stream);
+}
+
+}  // namespace tree
+}  // namespace wtq
