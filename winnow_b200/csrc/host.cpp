@@ -350,6 +350,16 @@ PyObject *tuple_of(std::initializer_list<at::Tensor> ts) {
   return r;
 }
 
+// `shape` of one buffer's elements from `at` on, which moves past them (a tensor of its own, without the
+// dispatcher: nine allocations or views of a plan cost as much as its kernel).
+at::Tensor cut(const at::Tensor &buffer, int64_t &at, at::IntArrayRef shape) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(), buffer.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(at);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+  at += (t.numel() + 63) / 64 * 64;
+  return t;
+}
+
 // rope(q, k, v, positions, table, q_weight, k_weight, eps, interleaved, out, status) -> (q, k[, v]), or None
 PyObject *rope(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -465,16 +475,17 @@ PyObject *plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
         !words(o[7], dev, {tokens}) || (parents.defined() && (!o[8].defined() || !words(o[8], dev, {B, Q, words_of}))))
       Py_RETURN_NONE;
   } else {
-    const auto opt = lengths.options();
-    o[0] = at::empty({B}, opt);
-    o[1] = at::empty({B}, opt);
-    o[2] = at::empty({1}, opt);
-    o[3] = at::empty({B + 1}, opt);
-    o[4] = at::empty({tokens}, opt);
-    o[5] = at::empty({tokens}, opt);
-    o[6] = at::empty({tokens, 1}, opt);
-    o[7] = at::empty({tokens}, opt);
-    if (parents.defined()) o[8] = at::empty({B, Q, words_of}, opt);
+    const at::Tensor buffer = at::empty({9 * 64 + 3 * B + 2 + 4 * tokens + B * Q * words_of}, lengths.options());
+    int64_t at = 0;
+    o[0] = cut(buffer, at, {B});
+    o[1] = cut(buffer, at, {B});
+    o[2] = cut(buffer, at, {1});
+    o[3] = cut(buffer, at, {B + 1});
+    o[4] = cut(buffer, at, {tokens});
+    o[5] = cut(buffer, at, {tokens});
+    o[6] = cut(buffer, at, {tokens, 1});
+    o[7] = cut(buffer, at, {tokens});
+    if (parents.defined()) o[8] = cut(buffer, at, {B, Q, words_of});
   }
   int32_t *p[9];
   for (int i = 0; i < 9; ++i) p[i] = o[i].defined() ? o[i].mutable_data_ptr<int32_t>() : nullptr;

@@ -103,8 +103,37 @@ __device__ __forceinline__ int table_row(const Params &p, int b, int i, bool rep
   return pos < p.table_rows ? pos : -1;
 }
 
+// A thread's two pieces of a weight vector (ones without weights).
+template <int V> __device__ __forceinline__ void load_weights(const void *w, int dtype, int at0, int at1, float (&x)[2 * V]) {
+  const int el = dtype == WTQ_F32 ? 4 : 2;
+  if (w == nullptr) {
+#pragma unroll
+    for (int j = 0; j < 2 * V; ++j) x[j] = 1.f;
+  } else if (16 / el == V && ((uintptr_t)w & 15) == 0) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4 *>((const char *)w + at0 * el));
+    const uint4 c = __ldg(reinterpret_cast<const uint4 *>((const char *)w + at1 * el));
+    if constexpr (V == 4) {
+      unpack<WTQ_F32>(a, x);
+      unpack<WTQ_F32>(c, x + V);
+    } else if (dtype == WTQ_F16) {
+      unpack<WTQ_F16>(a, x);
+      unpack<WTQ_F16>(c, x + V);
+    } else {
+      unpack<WTQ_BF16>(a, x);
+      unpack<WTQ_BF16>(c, x + V);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      x[j] = load_as_float(w, at0 + j, dtype);
+      x[V + j] = load_as_float(w, at1 + j, dtype);
+    }
+  }
+}
+
 // TPR threads a row (a power of two, at most 32); D, rot and D - rot are multiples of two pieces
-// and every row is 16-byte aligned.
+// and every row is 16-byte aligned.  The pieces of kBatch heads are read before the first is worked on.
+constexpr int kBatch = 4;
 template <int DT, int TPR, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) rows_kernel(Params p) {
   constexpr int V = Vec<DT>::kN;
@@ -115,56 +144,85 @@ __global__ void __launch_bounds__(256) rows_kernel(Params p) {
   // (threads of a warp stay together for the shuffles: a group past the end works on nothing)
   const bool real = token < (int64_t)p.B * p.n;
   const int first = real ? (int)(group - token * per_token) * p.heads_per_group : p.heads;
+  const int last = min(first + p.heads_per_group, p.heads);
   const int b = real ? (int)(token / p.n) : 0, i = real ? (int)(token - (int64_t)b * p.n) : 0;
   const int pairs = p.D / (2 * V), turned_pairs = p.rot / (2 * V);
   const bool has = lane_in_row < pairs, turns = lane_in_row < turned_pairs;
   // where this thread's two pieces start
   const int at0 = turns ? lane_in_row * V : p.rot + 2 * (lane_in_row - turned_pairs) * V;
   const int at1 = turns ? at0 + p.rot / 2 : at0 + V;
+  auto load = [&](int k, uint4 &a, uint4 &c) {
+    int head = first + k;
+    if (head >= last || !has) return;
+    const Side &sd = side_of(p, head);
+    const char *src = (const char *)sd.x + (b * sd.xb + head * sd.xh + i * sd.xt) * (16 / V);
+    a = *reinterpret_cast<const uint4 *>(src + at0 * (16 / V));
+    c = *reinterpret_cast<const uint4 *>(src + at1 * (16 / V));
+  };
+  uint4 raw[kBatch][2];
+  auto load_batch = [&](int k) {
+#pragma unroll
+    for (int e = 0; e < kBatch; ++e) {
+      raw[e][0] = raw[e][1] = make_uint4(0u, 0u, 0u, 0u);
+      if (k + e < p.heads_per_group) load(k + e, raw[e][0], raw[e][1]);
+    }
+  };
+  load_batch(0);
   const int row = real ? table_row(p, b, i, lane_in_row == 0 && first == 0) : -1;
   float c[V], s[V];               // of the pairs of both pieces (halves: of piece 0's elements)
 #pragma unroll
   for (int j = 0; j < V; ++j) c[j] = 1.f, s[j] = 0.f;
   if (turns && row >= 0) {
     const float *t = p.table + (int64_t)row * p.table_stride;
+    // interleaved: pairs at0 / 2 .. and at1 / 2 .. of V / 2 each
+    const int half = p.rot / 2, from0 = INTERLEAVED ? at0 / 2 : at0, from1 = INTERLEAVED ? at1 / 2 : at0 + V / 2;
+    if ((((uintptr_t)t | (uintptr_t)(half * 4)) & 15) == 0 && V / 2 % 4 == 0) {
+      *reinterpret_cast<float4 *>(c) = __ldg(reinterpret_cast<const float4 *>(t + from0));
+      *reinterpret_cast<float4 *>(s) = __ldg(reinterpret_cast<const float4 *>(t + half + from0));
+      if constexpr (V == 8) {
+        *reinterpret_cast<float4 *>(c + V / 2) = __ldg(reinterpret_cast<const float4 *>(t + from1));
+        *reinterpret_cast<float4 *>(s + V / 2) = __ldg(reinterpret_cast<const float4 *>(t + half + from1));
+      }
+    } else {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      // interleaved: pairs at0 / 2 .. and at1 / 2 .. of V / 2 each
-      const int pair = !INTERLEAVED ? at0 + j : j < V / 2 ? at0 / 2 + j : at1 / 2 + j - V / 2;
-      c[j] = __ldg(t + pair);
-      s[j] = __ldg(t + p.rot / 2 + pair);
+      for (int j = 0; j < V; ++j) {
+        const int pair = j < V / 2 ? from0 + j : from1 + j - V / 2;
+        c[j] = __ldg(t + pair);
+        s[j] = __ldg(t + half + pair);
+      }
     }
   }
-  const int last = real ? min(first + p.heads_per_group, p.heads) : p.heads;
-  const int steps = p.heads_per_group;
-#pragma unroll 2
-  for (int k = 0; k < steps; ++k) {
-    int head = first + k;
+  float weight[2 * V];
+  const void *held = nullptr;
+  bool any_held = false;
+  for (int k0 = 0; k0 < p.heads_per_group; k0 += kBatch) {
+   if (k0 > 0) load_batch(k0);
+#pragma unroll
+   for (int e = 0; e < kBatch; ++e) {
+    if (k0 + e >= p.heads_per_group) break;              // (the same for all)
+    int head = first + k0 + e;
     const bool work = head < last && has;
     if (!work) head = 0;
     const Side &sd = side_of(p, head);
     float x[2 * V];
-#pragma unroll
-    for (int j = 0; j < 2 * V; ++j) x[j] = 0.f;
-    if (work) {
-      const int64_t at = b * sd.xb + head * sd.xh + i * sd.xt;
-      const char *src = (const char *)sd.x + at * (16 / V);
-      unpack<DT>(*reinterpret_cast<const uint4 *>(src + at0 * (16 / V)), x);
-      unpack<DT>(*reinterpret_cast<const uint4 *>(src + at1 * (16 / V)), x + V);
+    unpack<DT>(raw[e][0], x);
+    unpack<DT>(raw[e][1], x + V);
+    if (work && (!any_held || held != sd.weight)) {
+      load_weights<V>(sd.weight, p.weight_dtype, at0, at1, weight);
+      held = sd.weight;
+      any_held = true;
     }
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < 2 * V; ++j) sum = fmaf(x[j], x[j], sum);
+    if (!work) sum = 0.f;
 #pragma unroll
     for (int o = TPR / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o, TPR);
     if (work) {
       if (sd.weight != nullptr) {
         const float r = 1.f / sqrtf(sum / (float)p.D + p.eps);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          x[j] *= r * load_as_float(sd.weight, at0 + j, p.weight_dtype);
-          x[V + j] *= r * load_as_float(sd.weight, at1 + j, p.weight_dtype);
-        }
+        for (int j = 0; j < 2 * V; ++j) x[j] *= r * weight[j];
       }
       if (sd.turned) {
         if (row < 0) {
@@ -186,11 +244,11 @@ __global__ void __launch_bounds__(256) rows_kernel(Params p) {
           }
         }
       }
-      const int64_t at = b * sd.ob + head * sd.oh + i * sd.ot;
-      char *dst = (char *)sd.out + at * (16 / V);
+      char *dst = (char *)sd.out + (b * sd.ob + head * sd.oh + i * sd.ot) * (16 / V);
       *reinterpret_cast<uint4 *>(dst + at0 * (16 / V)) = packed<DT>(x);
       *reinterpret_cast<uint4 *>(dst + at1 * (16 / V)) = packed<DT>(x + V);
     }
+   }
   }
 }
 
@@ -302,6 +360,8 @@ extern "C" int wtq_qk_norm_rope(const wtq_rope_side_t sides[3], int dtype, int w
     const int64_t room = (int64_t)device_sms() * 2048;
     const int64_t per_token = std::min<int64_t>(p.heads, std::max<int64_t>(1, (room + threads - 1) / threads));
     p.heads_per_group = (int)((p.heads + per_token - 1) / per_token);
+    if (p.heads_per_group > rope::kBatch)                // whole batches
+      p.heads_per_group = (p.heads_per_group + rope::kBatch - 1) / rope::kBatch * rope::kBatch;
     if (dtype == WTQ_F32) rope::launch_width<WTQ_F32>(p, tpr, interleaved, stream);
     else if (dtype == WTQ_F16) rope::launch_width<WTQ_F16>(p, tpr, interleaved, stream);
     else rope::launch_width<WTQ_BF16>(p, tpr, interleaved, stream);

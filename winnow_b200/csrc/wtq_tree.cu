@@ -66,6 +66,7 @@ __global__ void __launch_bounds__(kRowThreads) rotate_kernel(Params p) {
 __global__ void __launch_bounds__(kRowThreads) join_kernel(Params p) {
   extern __shared__ float a[];
   __shared__ int prefix[kMaxBatch + 1];
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
   tile_prefix(p, prefix);
   const long long share = run_length(p, prefix);
   const int64_t rows = (int64_t)p.B * p.Q * p.Hq, row0 = (int64_t)blockIdx.x * kRowBlock;
@@ -141,49 +142,83 @@ inline size_t scan_bytes(int D) {
   return sizeof(float) * ((size_t)(kScanRows + 2 * kScanTile) * scan_pitch(D) + kScanRows * (kScanTile + 4) + kScanRows);
 }
 
-// A tile's rows of one side as centroid times norm; rows past the end and of pages outside the pool are zeros.
-__device__ __forceinline__ void decode_rows(const Params &p, const DecodeSideDev &sd, const int32_t *table, int h, int tok0,
-                                            int end, float *to, int pitch, int padded) {
-  const int per = kScanThreads / kScanTile;                   // threads a row
-  const int r = threadIdx.x / per, tok = tok0 + r;
-  const uint8_t *row = nullptr;
-  float norm = 0.f;
+// Eight codes of `bw` bits, whole bytes whatever the width (`words`: 4- or 8-bit codes on 4-byte borders).
+__device__ __forceinline__ uint64_t eight_codes(const uint8_t *src, int bw, bool words) {
+  uint64_t w = 0;
+  if (words) {
+    w = __ldg(reinterpret_cast<const uint32_t *>(src));
+    if (bw == 8) w |= (uint64_t)__ldg(reinterpret_cast<const uint32_t *>(src) + 1) << 32;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < bw) w |= (uint64_t)__ldg(src + i) << (8 * i);
+  }
+  return w;
+}
+
+// A tile's rows of both sides as centroid times norm; rows past the end and of pages outside the pool are
+// zeros.  Eight threads a row; all of a thread's codes are read before the first is looked up.
+__device__ __forceinline__ void decode_rows(const Params &p, const int32_t *table, int h, int tok0, int end, const float *cents,
+                                            float *ks, float *vs, int pitch, int padded) {
+  constexpr int kPer = kScanThreads / kScanTile;
+  const int r = threadIdx.x / kPer, tok = tok0 + r, d_first = 8 * (threadIdx.x % kPer);
+  const uint8_t *row[2] = {nullptr, nullptr};
+  float norm[2] = {0.f, 0.f};
   if (tok < end) {
     const int page = table[tok / p.S], slot = tok % p.S;
     if ((uint32_t)page < (uint32_t)p.P) {
-      row = sd.pages + (int64_t)page * sd.page_stride + h * sd.head_stride + (int64_t)slot * sd.nb;
-      norm = __half2float(sd.norms[(int64_t)page * sd.norm_page_stride + h * sd.norm_head_stride + slot]);
-    } else if (p.status && threadIdx.x % per == 0) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const DecodeSideDev &sd = s ? p.v : p.k;
+        row[s] = sd.pages + (int64_t)page * sd.page_stride + h * sd.head_stride + (int64_t)slot * sd.nb;
+        norm[s] = __half2float(sd.norms[(int64_t)page * sd.norm_page_stride + h * sd.norm_head_stride + slot]);
+      }
+    } else if (p.status && threadIdx.x % kPer == 0) {
       atomicOr(p.status, WTQ_STATUS_BAD_PAGE);
     }
   }
-  // eight codes are bw bytes: whole bytes whatever the width
-  for (int d0 = 8 * (threadIdx.x % per); d0 < padded; d0 += 8 * per) {
-    float x[8];
-    if (row != nullptr && d0 + 8 <= p.D) {
-      uint64_t w = 0;
-      const uint8_t *src = row + d0 / 8 * sd.bw;
-      for (int i = 0; i < sd.bw; ++i) w |= (uint64_t)src[i] << (8 * i);
+  constexpr int kMost = 256 / (8 * kPer);                     // groups of eight codes of a thread
+  uint64_t w[2][kMost];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] = __ldg(sd.centroids + (int)(w & ((1u << sd.bw) - 1u))) * norm;
-        w >>= sd.bw;
-      }
-    } else {
+  for (int k = 0; k < kMost; ++k)
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        x[i] = row != nullptr && d0 + i < p.D ? __ldg(sd.centroids + extract_code(row, d0 + i, sd.bw, sd.nb)) * norm : 0.f;
+    for (int s = 0; s < 2; ++s) {
+      const DecodeSideDev &sd = s ? p.v : p.k;
+      const int d0 = d_first + 8 * kPer * k;
+      w[s][k] = 0;
+      if (row[s] != nullptr && d0 + 8 <= p.D)
+        w[s][k] = eight_codes(row[s] + d0 / 8 * sd.bw, sd.bw, sd.bw % 4 == 0 && ((uintptr_t)row[s] & 3) == 0);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (d0 + i < padded) to[r * pitch + d0 + i] = x[i];
-  }
+  for (int k = 0; k < kMost; ++k)
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const DecodeSideDev &sd = s ? p.v : p.k;
+      const int d0 = d_first + 8 * kPer * k;
+      float *to = (s ? vs : ks) + r * pitch + d0;
+      if (d0 >= padded) continue;
+      uint64_t x = w[s][k];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int code = (int)(x & ((1u << sd.bw) - 1u));
+        x >>= sd.bw;
+        if (d0 + 8 <= p.D) to[i] = row[s] ? cents[256 * s + code] * norm[s] : 0.f;
+        else if (d0 + i < padded)                             // the last, odd group
+          to[i] = row[s] && d0 + i < p.D ? cents[256 * s + extract_code(row[s], d0 + i, sd.bw, sd.nb)] * norm[s] : 0.f;
+      }
+    }
 }
 
 template <int NJ>
 __global__ void __launch_bounds__(kScanThreads) scan_kernel(Params p) {
   extern __shared__ __align__(16) float smem[];
   __shared__ int prefix[kMaxBatch + 1];
+  __shared__ float cents[512];
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  for (int e = threadIdx.x; e < 512; e += kScanThreads) {
+    const DecodeSideDev &sd = e < 256 ? p.k : p.v;
+    cents[e] = (e & 255) < 1 << sd.bw ? __ldg(sd.centroids + (e & 255)) : 0.f;
+  }
   const int pitch = scan_pitch(p.D), padded = (p.D + 3) / 4 * 4;
   float *qs = smem, *ks = qs + kScanRows * pitch, *vs = ks + kScanTile * pitch, *ps = vs + kScanTile * pitch;
   float *factor = ps + kScanRows * (kScanTile + 4);
@@ -193,20 +228,25 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(Params p) {
   tile_prefix(p, prefix);
   const long long share = run_length(p, prefix), all = (long long)prefix[p.B] * p.row_blocks * p.Hkv;
   const long long begin = share * blockIdx.x, end = min(all, begin + share);
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");       // the rotated queries
   for (long long x = begin; x < end;) {
     const Piece c = piece_at(p, prefix, x, begin, end);
     x += c.last - c.first;
     const int L = length_of(p, c.b), hist = L - p.Q, row0 = c.rb * p.rows;
     const int32_t *table = p.page_table + (int64_t)c.b * p.table_stride;
     __syncthreads();
-    for (int e = tid; e < kScanRows * padded; e += kScanThreads) {
-      const int r = e / padded, d = e - r * padded, qr = row0 + r;
-      float v = 0.f;
-      if (qr < p.R && d < p.D) {
-        const int i = qr / p.n_rep, head = c.h * p.n_rep + qr - i * p.n_rep;
-        v = p.q_rot[(((int64_t)c.b * p.Q + i) * p.Hq + head) * p.D + d];
+    {
+      const int r = tid >> 2, qr = row0 + r;                  // four threads a row
+      const int i = qr / p.n_rep, head = c.h * p.n_rep + qr - i * p.n_rep;
+      const float *from = p.q_rot + (((int64_t)c.b * p.Q + i) * p.Hq + head) * p.D;
+      if (p.D % 4 == 0) {
+#pragma unroll 4
+        for (int d = 4 * (tid & 3); d < padded; d += 16)
+          *reinterpret_cast<float4 *>(qs + r * pitch + d) =
+              qr < p.R ? *reinterpret_cast<const float4 *>(from + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+      } else {
+        for (int d = tid & 3; d < padded; d += 4) qs[r * pitch + d] = qr < p.R && d < p.D ? from[d] : 0.f;
       }
-      qs[r * pitch + d] = v;
     }
     float m[8], l[8];                                     // of rows 8 warp .. 8 warp + 7
     bool dead[8];
@@ -225,8 +265,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(Params p) {
     for (int tile = c.first; tile < c.last; ++tile) {
       const int tok0 = tile * kScanTile;
       __syncthreads();                                    // the last tile's rows have been used
-      decode_rows(p, p.k, table, c.h, tok0, L, ks, pitch, padded);
-      decode_rows(p, p.v, table, c.h, tok0, L, vs, pitch, padded);
+      decode_rows(p, table, c.h, tok0, L, cents, ks, vs, pitch, padded);
       __syncthreads();
       float s[4][2] = {};
       for (int d = 0; d < padded; d += 4) {
@@ -343,9 +382,7 @@ template <int NJ> int launch_scan(const Params &p, cudaStream_t stream) {
     if (e != cudaSuccess) return check_cuda(e, "wtq_tree: shared memory opt-in");
     opted_in[dev & 63].store(true, std::memory_order_release);
   }
-  scan_kernel<NJ><<<p.blocks, kScanThreads, scan_bytes(p.D), stream>>>(p);
-  note_launches(1);
-  return check_cuda(cudaGetLastError(), "wtq_tree scan launch");
+  return launch_behind(scan_kernel<NJ>, p.blocks, kScanThreads, scan_bytes(p.D), stream, "wtq_tree scan launch", p);
 }
 
 size_t round_up(size_t x) { return (x + 255) / 256 * 256; }
@@ -415,7 +452,7 @@ extern "C" int wtq_tree(const void *q, int dtype, const int64_t q_strides[3], vo
   p.tile = umma ? tree::kUmmaTile : tree::kScanTile;
   p.row_blocks = (p.R + p.rows - 1) / p.rows;
   p.blocks = tree::scan_blocks(umma, D);
-  p.least = umma ? 2 : 1;
+  p.least = 2;
   const int el = dtype == WTQ_F32 ? 4 : 2;
   for (int b0 = 0; b0 < B; b0 += tree::kMaxBatch) {
     p.B = std::min(B - b0, tree::kMaxBatch);

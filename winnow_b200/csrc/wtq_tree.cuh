@@ -123,6 +123,26 @@ __device__ __forceinline__ bool padding(const int32_t *words, int Q) {
   return any == 0;
 }
 
+// Launch behind the kernel ahead in the stream: its blocks may start, and set themselves up, while that
+// one's last blocks run; what depends on it comes after griddepcontrol.wait.
+template <typename... Kernel, typename... Args>
+int launch_behind(void (*kernel)(Kernel...), int blocks, int threads, size_t bytes, cudaStream_t stream, const char *what,
+                  Args... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  note_launches(1);
+  return check_cuda(e, what);
+}
+
 bool on_tensor_cores(const wtq_side_t &k, const wtq_side_t &v, int dtype, int D, int S);
 int launch_scan_umma(const Params &p, cudaStream_t stream);
 bool rows_on_tensor_cores(const Params &p);

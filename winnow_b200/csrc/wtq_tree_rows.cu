@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms) 
     if (p.status && tid == 0) atomicOr(p.status, WTQ_STATUS_LAYOUT);
     return;
   }
+  if (!JOIN) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   constexpr int kPieces = D / 8;
   const float *Pi = JOIN ? p.v.Pi : p.k.Pi;
   if (warp == 0) {
@@ -113,6 +114,7 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms) 
   if constexpr (JOIN) {
     tile_prefix(p, prefix);
     share = run_length(p, prefix);
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");   // the states
   }
   // ---- the rows: kPieces lanes a row, several rows of a warp at a time ------------------------------
   const int64_t rows = (int64_t)p.B * p.Q * p.Hq, row0 = (int64_t)blockIdx.x * kRows;
@@ -193,17 +195,15 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms) 
           const float w = m == -INFINITY ? 0.f : exp2f(m - top);
           if (w > 0.f) sum = fmaf(w, p.part_l[state(c)], sum);
           const int last = min(kPieces, c1 - from + 1);
-#pragma unroll 4
-          for (int e = 0; e < last; ++e) {
-            const float we = __shfl_sync(group, w, lane / kPieces * kPieces + e);
-            if (we > 0.f) add(p.part_acc + state(from + e) * D, we);
-          }
+#pragma unroll 8
+          for (int e = 0; e < last; ++e)                    // (a live row's accumulators are all written)
+            add(p.part_acc + state(from + e) * D, __shfl_sync(group, w, lane / kPieces * kPieces + e));
         }
 #pragma unroll
         for (int o = kPieces / 2; o; o >>= 1) sum += __shfl_xor_sync(group, sum, o);
         const float f = sum > 0.f ? 1.f / sum : 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= f;
+        for (int e = 0; e < 8; ++e) x[e] = sum > 0.f ? x[e] * f : 0.f;
       }
     }
     float most = 0.f, inverse;
@@ -304,10 +304,11 @@ template <bool JOIN, int D> int launch(const Params &p, cudaStream_t stream) {
     opted_in[dev & 63].store(true, std::memory_order_release);
   }
   const int64_t all = (int64_t)p.B * p.Q * p.Hq;
-  product_kernel<JOIN, D><<<(unsigned)((all + kRows - 1) / kRows), kThreads, M::kBytes, stream>>>(
-      p, JOIN || p.dtype == WTQ_F32 ? 3 : 2);
+  const int blocks = (int)((all + kRows - 1) / kRows), terms = JOIN || p.dtype == WTQ_F32 ? 3 : 2;
+  if (JOIN) return launch_behind(product_kernel<JOIN, D>, blocks, kThreads, M::kBytes, stream, "wtq_tree join launch", p, terms);
+  product_kernel<JOIN, D><<<blocks, kThreads, M::kBytes, stream>>>(p, terms);
   note_launches(1);
-  return check_cuda(cudaGetLastError(), "wtq_tree product launch");
+  return check_cuda(cudaGetLastError(), "wtq_tree rotate launch");
 }
 
 }  // namespace rows

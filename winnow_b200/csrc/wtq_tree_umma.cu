@@ -304,6 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(Params p) {
     if (p.status && tid == 0) atomicOr(p.status, WTQ_STATUS_LAYOUT);
     return;
   }
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   int *prefix = reinterpret_cast<int *>(dyn_smem + (kPrefix - (uint32_t)__cvta_generic_to_shared(dyn_smem)));
   for (int e = tid; e < M::kEntries * 64; e += kThreads)
     sts32(mma::kLutAddr + 4u * e, mma::lut_word(e, BWK, BWV, p.k.centroids, p.v.centroids));
@@ -355,6 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(Params p) {
                    o_addr = tmem + lanes + kColO + 128u * st;
     int n = 0;                                              // units of this stream so far
     bool ok = true;
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");   // the rotated queries (all else is there already)
     for (long long x = begin; x < end;) {
       const Piece c = piece_at(p, prefix, x, begin, end);
       const int nt = c.last - c.first;
@@ -608,9 +610,7 @@ template <int BWK, int BWV, int D> int launch(const Params &p, cudaStream_t stre
     if (e != cudaSuccess) return check_cuda(e, "wtq_tree: shared memory opt-in");
     opted_in[dev & 63].store(true, std::memory_order_release);
   }
-  scan_kernel<BWK, BWV, D><<<p.blocks, kThreads, M::kDynamic, stream>>>(p);
-  note_launches(1);
-  return check_cuda(cudaGetLastError(), "wtq_tree scan launch");
+  return launch_behind(scan_kernel<BWK, BWV, D>, p.blocks, kThreads, M::kDynamic, stream, "wtq_tree scan launch", p);
 }
 template <int D> int launch_widths(const Params &p, cudaStream_t stream) {
   if (p.k.bw == 4 && p.v.bw == 4) return launch<4, 4, D>(p, stream);
