@@ -10,10 +10,12 @@
 // A group of threads holds a row of a head in registers: thread c of the group two pieces of 16
 // bytes, piece c of the rotated part's first half and the piece of its second half that it turns
 // with (an interleaved pair never leaves a piece; the unrotated tail is dealt two pieces to a
-// thread too), so the rotation needs no exchange and the norm a few shuffles.  A group keeps a
-// token's table row in registers and walks over heads; how many depends on the call: with few
-// tokens a head each, which is the shortest chain, with many all of a token's heads, which reads
-// the table once.  Bound by HBM at prompts and by the launch at single tokens.
+// thread too), so the rotation needs no exchange and the norm a few shuffles.  A block takes adjacent
+// tokens and a run of heads, the same for all its groups: the table's rows and a side's weights stay in
+// registers, sides change for the whole block at once, and rows of a head are written side by side.
+// How many heads depends on the call: one with few tokens, which is the shortest chain, all of them
+// with many, which reads the table once.  Arithmetic is on two values at a time (f32x2).
+// Bound by HBM at prompts and by the launch at single tokens.
 #include <algorithm>
 
 #include "wtq_common.cuh"
@@ -47,35 +49,47 @@ struct Params {
 template <int DT> struct Vec {
   static constexpr int kN = DT == WTQ_F32 ? 4 : 8;      // elements of 16 bytes
 };
-template <int DT> __device__ __forceinline__ void unpack(const uint4 &v, float *x) {
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 16 bytes as pairs of fp32 values and back.
+template <int DT> __device__ __forceinline__ void unpack(const uint4 &v, uint64_t *x) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   if constexpr (DT == WTQ_F32) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float2 f;
-      if constexpr (DT == WTQ_F16) f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-      else f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w[i]));
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
-  }
-}
-template <int DT> __device__ __forceinline__ uint4 packed(const float *x) {
-  uint32_t w[4];
-  if constexpr (DT == WTQ_F32) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(x[i]);
+    for (int i = 0; i < 2; ++i) x[i] = pair(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (DT == WTQ_F16) {
-        const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        x[i] = pair(f.x, f.y);
+      } else {
+        x[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+      }
+    }
+  }
+}
+template <int DT> __device__ __forceinline__ uint4 packed(const uint64_t *x) {
+  uint32_t w[4];
+  if constexpr (DT == WTQ_F32) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 f = halves(x[i]);
+      w[2 * i] = __float_as_uint(f.x);
+      w[2 * i + 1] = __float_as_uint(f.y);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = halves(x[i]);
+      if constexpr (DT == WTQ_F16) {
+        const __half2 h = __floats2half2_rn(f.x, f.y);
         w[i] = *reinterpret_cast<const uint32_t *>(&h);
       } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
         w[i] = *reinterpret_cast<const uint32_t *>(&h);
       }
     }
@@ -103,152 +117,149 @@ __device__ __forceinline__ int table_row(const Params &p, int b, int i, bool rep
   return pos < p.table_rows ? pos : -1;
 }
 
-// A thread's two pieces of a weight vector (ones without weights).
-template <int V> __device__ __forceinline__ void load_weights(const void *w, int dtype, int at0, int at1, float (&x)[2 * V]) {
-  const int el = dtype == WTQ_F32 ? 4 : 2;
-  if (w == nullptr) {
-#pragma unroll
-    for (int j = 0; j < 2 * V; ++j) x[j] = 1.f;
-  } else if (16 / el == V && ((uintptr_t)w & 15) == 0) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4 *>((const char *)w + at0 * el));
-    const uint4 c = __ldg(reinterpret_cast<const uint4 *>((const char *)w + at1 * el));
-    if constexpr (V == 4) {
-      unpack<WTQ_F32>(a, x);
-      unpack<WTQ_F32>(c, x + V);
-    } else if (dtype == WTQ_F16) {
-      unpack<WTQ_F16>(a, x);
-      unpack<WTQ_F16>(c, x + V);
-    } else {
-      unpack<WTQ_BF16>(a, x);
-      unpack<WTQ_BF16>(c, x + V);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      x[j] = load_as_float(w, at0 + j, dtype);
-      x[V + j] = load_as_float(w, at1 + j, dtype);
-    }
-  }
-}
-
 // TPR threads a row (a power of two, at most 32); D, rot and D - rot are multiples of two pieces
 // and every row is 16-byte aligned.  The pieces of kBatch heads are read before the first is worked on.
-constexpr int kBatch = 4;
+constexpr int kThreads = 128, kBatch = 2;
 template <int DT, int TPR, bool INTERLEAVED>
-__global__ void __launch_bounds__(256) rows_kernel(Params p) {
-  constexpr int V = Vec<DT>::kN;
+__global__ void __launch_bounds__(kThreads, 5) rows_kernel(Params p) {
+  constexpr int V = Vec<DT>::kN, N = V / 2;               // values and pairs of a piece
+  constexpr int kEl = 16 / V;
   const int lane_in_row = threadIdx.x % TPR;
-  const int64_t group = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
-  const int per_token = (p.heads + p.heads_per_group - 1) / p.heads_per_group;
-  const int64_t token = group / per_token;
+  const int64_t token = (int64_t)blockIdx.x * (kThreads / TPR) + threadIdx.x / TPR;
+  const int first = blockIdx.y * p.heads_per_group, last = min(first + p.heads_per_group, p.heads);
   // (threads of a warp stay together for the shuffles: a group past the end works on nothing)
   const bool real = token < (int64_t)p.B * p.n;
-  const int first = real ? (int)(group - token * per_token) * p.heads_per_group : p.heads;
-  const int last = min(first + p.heads_per_group, p.heads);
-  const int b = real ? (int)(token / p.n) : 0, i = real ? (int)(token - (int64_t)b * p.n) : 0;
+  const int b = real ? (int)((uint32_t)token / (uint32_t)p.n) : 0, i = real ? (int)(token - (int64_t)b * p.n) : 0;
   const int pairs = p.D / (2 * V), turned_pairs = p.rot / (2 * V);
-  const bool has = lane_in_row < pairs, turns = lane_in_row < turned_pairs;
+  const bool work = real && lane_in_row < pairs, turns = lane_in_row < turned_pairs;
   // where this thread's two pieces start
   const int at0 = turns ? lane_in_row * V : p.rot + 2 * (lane_in_row - turned_pairs) * V;
   const int at1 = turns ? at0 + p.rot / 2 : at0 + V;
-  auto load = [&](int k, uint4 &a, uint4 &c) {
-    int head = first + k;
-    if (head >= last || !has) return;
-    const Side &sd = side_of(p, head);
-    const char *src = (const char *)sd.x + (b * sd.xb + head * sd.xh + i * sd.xt) * (16 / V);
-    a = *reinterpret_cast<const uint4 *>(src + at0 * (16 / V));
-    c = *reinterpret_cast<const uint4 *>(src + at1 * (16 / V));
+  // the side that the walk stands in: rows of this token, head by head
+  int side = -1, left = 0;
+  const char *src = nullptr;
+  char *dst = nullptr;
+  int64_t src_step = 0, dst_step = 0;
+  auto enter = [&](int s, int head) {                     // the same for the whole block
+    side = s;
+    const Side &sd = p.side[s];
+    left = sd.heads - head;
+    src = (const char *)sd.x + (b * sd.xb + head * sd.xh + i * sd.xt) * kEl;
+    dst = (char *)sd.out + (b * sd.ob + head * sd.oh + i * sd.ot) * kEl;
+    src_step = sd.xh * kEl;
+    dst_step = sd.oh * kEl;
   };
-  uint4 raw[kBatch][2];
-  auto load_batch = [&](int k) {
+  {
+    int head = first, s = 0;
+    while (head >= p.side[s].heads) head -= p.side[s++].heads;
+    enter(s, head);
+  }
+  const int row = real ? table_row(p, b, i, lane_in_row == 0 && blockIdx.y == 0) : -1;
+  // cosines and sines: halves: of piece 0's values; interleaved: (c, c) and (-s, s) of both pieces' pairs
+  uint64_t cs[INTERLEAVED ? 2 * N : N], sn[INTERLEAVED ? 2 * N : N], minus[INTERLEAVED ? 1 : N];
 #pragma unroll
-    for (int e = 0; e < kBatch; ++e) {
-      raw[e][0] = raw[e][1] = make_uint4(0u, 0u, 0u, 0u);
-      if (k + e < p.heads_per_group) load(k + e, raw[e][0], raw[e][1]);
-    }
-  };
-  load_batch(0);
-  const int row = real ? table_row(p, b, i, lane_in_row == 0 && first == 0) : -1;
-  float c[V], s[V];               // of the pairs of both pieces (halves: of piece 0's elements)
+  for (int j = 0; j < (INTERLEAVED ? 2 * N : N); ++j) cs[j] = twice(1.f), sn[j] = 0;
 #pragma unroll
-  for (int j = 0; j < V; ++j) c[j] = 1.f, s[j] = 0.f;
+  for (int j = 0; j < (INTERLEAVED ? 1 : N); ++j) minus[j] = 0;
   if (turns && row >= 0) {
-    const float *t = p.table + (int64_t)row * p.table_stride;
-    // interleaved: pairs at0 / 2 .. and at1 / 2 .. of V / 2 each
-    const int half = p.rot / 2, from0 = INTERLEAVED ? at0 / 2 : at0, from1 = INTERLEAVED ? at1 / 2 : at0 + V / 2;
-    if ((((uintptr_t)t | (uintptr_t)(half * 4)) & 15) == 0 && V / 2 % 4 == 0) {
-      *reinterpret_cast<float4 *>(c) = __ldg(reinterpret_cast<const float4 *>(t + from0));
-      *reinterpret_cast<float4 *>(s) = __ldg(reinterpret_cast<const float4 *>(t + half + from0));
-      if constexpr (V == 8) {
-        *reinterpret_cast<float4 *>(c + V / 2) = __ldg(reinterpret_cast<const float4 *>(t + from1));
-        *reinterpret_cast<float4 *>(s + V / 2) = __ldg(reinterpret_cast<const float4 *>(t + half + from1));
-      }
-    } else {
+    const float *t = p.table + (int64_t)row * p.table_stride, *u = t + p.rot / 2;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int pair = j < V / 2 ? from0 + j : from1 + j - V / 2;
-        c[j] = __ldg(t + pair);
-        s[j] = __ldg(t + half + pair);
+    for (int j = 0; j < (INTERLEAVED ? 2 * N : N); ++j) {
+      if constexpr (INTERLEAVED) {
+        const int k = j < N ? at0 / 2 + j : at1 / 2 + j - N;
+        const float c = __ldg(t + k), s = __ldg(u + k);
+        cs[j] = twice(c);
+        sn[j] = pair(-s, s);
+      } else {
+        const int k = at0 + 2 * j;
+        const float s0 = __ldg(u + k), s1 = __ldg(u + k + 1);
+        cs[j] = pair(__ldg(t + k), __ldg(t + k + 1));
+        sn[j] = pair(s0, s1);
+        minus[j] = pair(-s0, -s1);
       }
     }
   }
-  float weight[2 * V];
-  const void *held = nullptr;
-  bool any_held = false;
-  for (int k0 = 0; k0 < p.heads_per_group; k0 += kBatch) {
-   if (k0 > 0) load_batch(k0);
+  uint64_t weight[2 * N];
+  int weighed = -1;                                       // the side whose weights these are
+  for (int head = first; head < last; head += kBatch) {
+    uint4 raw[kBatch][2];
+    char *to[kBatch];
+    int of[kBatch];
 #pragma unroll
-   for (int e = 0; e < kBatch; ++e) {
-    if (k0 + e >= p.heads_per_group) break;              // (the same for all)
-    int head = first + k0 + e;
-    const bool work = head < last && has;
-    if (!work) head = 0;
-    const Side &sd = side_of(p, head);
-    float x[2 * V];
-    unpack<DT>(raw[e][0], x);
-    unpack<DT>(raw[e][1], x + V);
-    if (work && (!any_held || held != sd.weight)) {
-      load_weights<V>(sd.weight, p.weight_dtype, at0, at1, weight);
-      held = sd.weight;
-      any_held = true;
-    }
-    float sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < 2 * V; ++j) sum = fmaf(x[j], x[j], sum);
-    if (!work) sum = 0.f;
-#pragma unroll
-    for (int o = TPR / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o, TPR);
-    if (work) {
-      if (sd.weight != nullptr) {
-        const float r = 1.f / sqrtf(sum / (float)p.D + p.eps);
-#pragma unroll
-        for (int j = 0; j < 2 * V; ++j) x[j] *= r * weight[j];
+    for (int e = 0; e < kBatch; ++e) {
+      of[e] = -1;
+      if (head + e >= last) continue;
+      while (left == 0) enter(side + 1, 0);
+      of[e] = side;
+      to[e] = dst;
+      if (work) {
+        raw[e][0] = *reinterpret_cast<const uint4 *>(src + at0 * kEl);
+        raw[e][1] = *reinterpret_cast<const uint4 *>(src + at1 * kEl);
+      } else {
+        raw[e][0] = raw[e][1] = make_uint4(0u, 0u, 0u, 0u);
       }
-      if (sd.turned) {
+      src += src_step;
+      dst += dst_step;
+      --left;
+    }
+#pragma unroll
+    for (int e = 0; e < kBatch; ++e) {
+      if (of[e] < 0) continue;                            // (the same for the whole block)
+      const void *w = p.side[of[e]].weight;
+      if (of[e] < 2) {
+        uint64_t x[2 * N];
+        unpack<DT>(raw[e][0], x);
+        unpack<DT>(raw[e][1], x + N);
+        if (w != nullptr) {
+          if (weighed != of[e] && work) {
+#pragma unroll
+            for (int j = 0; j < 2 * N; ++j) {
+              const int k = (j < N ? at0 : at1 - V) + 2 * j;
+              weight[j] = pair(load_as_float(w, k, p.weight_dtype), load_as_float(w, k + 1, p.weight_dtype));
+            }
+          }
+          weighed = of[e];
+          uint64_t sums = 0;
+#pragma unroll
+          for (int j = 0; j < 2 * N; ++j) fma2(sums, x[j], x[j]);
+          const float2 both = halves(sums);
+          float sum = both.x + both.y;
+#pragma unroll
+          for (int o = TPR / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o, TPR);
+          const uint64_t r = twice(rsqrtf(sum / (float)p.D + p.eps));
+#pragma unroll
+          for (int j = 0; j < 2 * N; ++j) x[j] = mul2(mul2(x[j], weight[j]), r);
+        }
         if (row < 0) {
 #pragma unroll
-          for (int j = 0; j < 2 * V; ++j) x[j] = 0.f;
-        } else if (INTERLEAVED) {
+          for (int j = 0; j < 2 * N; ++j) x[j] = 0;
+        } else if (INTERLEAVED && turns) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float a = x[2 * j], d = x[2 * j + 1];
-            x[2 * j] = a * c[j] - d * s[j];
-            x[2 * j + 1] = d * c[j] + a * s[j];
+          for (int j = 0; j < 2 * N; ++j) {
+            const float2 v = halves(x[j]);
+            constexpr int kTop = INTERLEAVED ? 2 * N - 1 : 0;
+            uint64_t y = mul2(pair(v.y, v.x), sn[j < kTop ? j : kTop]);
+            fma2(y, x[j], cs[j < kTop ? j : kTop]);
+            x[j] = y;
           }
-        } else {
+        } else if (!INTERLEAVED && turns) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float a = x[j], d = x[V + j];
-            x[j] = a * c[j] - d * s[j];
-            x[V + j] = d * c[j] + a * s[j];
+          for (int j = 0; j < N; ++j) {
+            uint64_t y = mul2(x[N + j], minus[INTERLEAVED ? 0 : j]), z = mul2(x[j], sn[j]);
+            fma2(y, x[j], cs[j]);
+            fma2(z, x[N + j], cs[j]);
+            x[j] = y;
+            x[N + j] = z;
           }
         }
+        raw[e][0] = packed<DT>(x);
+        raw[e][1] = packed<DT>(x + N);
       }
-      char *dst = (char *)sd.out + (b * sd.ob + head * sd.oh + i * sd.ot) * (16 / V);
-      *reinterpret_cast<uint4 *>(dst + at0 * (16 / V)) = packed<DT>(x);
-      *reinterpret_cast<uint4 *>(dst + at1 * (16 / V)) = packed<DT>(x + V);
+      if (work) {
+        *reinterpret_cast<uint4 *>(to[e] + at0 * kEl) = raw[e][0];
+        *reinterpret_cast<uint4 *>(to[e] + at1 * kEl) = raw[e][1];
+      }
     }
-   }
   }
 }
 
@@ -295,11 +306,10 @@ __global__ void __launch_bounds__(128) any_kernel(Params p, int dtype, int inter
 
 template <int DT, int TPR>
 void launch(const Params &p, bool interleaved, cudaStream_t stream) {
-  const int per_token = (p.heads + p.heads_per_group - 1) / p.heads_per_group;
-  const int64_t groups = (int64_t)p.B * p.n * per_token;
-  const unsigned blocks = (unsigned)((groups + 256 / TPR - 1) / (256 / TPR));
-  if (interleaved) rows_kernel<DT, TPR, true><<<blocks, 256, 0, stream>>>(p);
-  else rows_kernel<DT, TPR, false><<<blocks, 256, 0, stream>>>(p);
+  const int64_t tokens = (int64_t)p.B * p.n;
+  const dim3 grid((unsigned)((tokens * TPR + kThreads - 1) / kThreads), (p.heads + p.heads_per_group - 1) / p.heads_per_group);
+  if (interleaved) rows_kernel<DT, TPR, true><<<grid, kThreads, 0, stream>>>(p);
+  else rows_kernel<DT, TPR, false><<<grid, kThreads, 0, stream>>>(p);
 }
 template <int DT>
 void launch_width(const Params &p, int tpr, bool interleaved, cudaStream_t stream) {
@@ -337,6 +347,7 @@ extern "C" int wtq_qk_norm_rope(const wtq_rope_side_t sides[3], int dtype, int w
     d = {w.x, w.out, w.strides[0], w.strides[1], w.strides[2], w.out_strides[0], w.out_strides[1],
          w.out_strides[2], w.weight, w.heads, s < 2};
     p.heads += w.heads;
+    if (p.heads > 65535) return fail(WTQ_ERR_ARG, "wtq_qk_norm_rope: too many heads");
     if (w.heads == 0 || B == 0 || n == 0) continue;
     if (!w.x || !w.out) return fail(WTQ_ERR_ARG, "wtq_qk_norm_rope: null input or output");
     vec = vec && ((uintptr_t)w.x % 16 | (uintptr_t)w.out % 16) == 0;
