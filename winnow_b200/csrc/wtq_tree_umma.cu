@@ -53,11 +53,10 @@ constexpr uint32_t kRawFull = kTileFree + 16 * kStages, kRawFree = kRawFull + 16
 constexpr uint32_t kSFull = kRawFree + 16 * kMostRaw, kSFree = kSFull + 16, kPFull = kSFree + 16,
                    kODone = kPFull + 16;                                   // [stream]
 constexpr uint32_t kQFull = kODone + 16, kLast = kQFull + 8, kTmemSlot = kLast + 8, kAbort = kTmemSlot + 4;
-constexpr uint32_t kValid = kAbort + 4;                                    // [side][raw tile]: tokens of it that exist
 constexpr uint32_t kPrefix = kBase + 512;                                  // kMaxBatch + 1 words
 constexpr uint32_t kStates = kPrefix + 4 * (kMaxBatch + 4);                // [stream][m, l of a half, l of the other][row]
 constexpr uint32_t kVTile = 16384;
-static_assert(kValid + 8 * kMostRaw <= kPrefix && kStates + 6 * kRows * 4 <= kVTile, "low region");
+static_assert(kAbort + 4 <= kPrefix && kStates + 6 * kRows * 4 <= kVTile, "low region");
 static_assert(kVTile + kStages * kTile * 256 <= mma::kLutAddr, "value tiles end where the tables begin");
 // tensor memory columns
 constexpr uint32_t kColQ = 0, kColS = 64, kColP = 192, kColO = 256, kCols = 512;   // S + 64, P + 32, O + 128 per stream
@@ -82,9 +81,9 @@ template <int BWK, int BWV, int D> struct Map {
   static constexpr uint32_t kIdescPV = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
 };
 
-// 16 bytes to shared memory, zeros where `there` is false (`from` is then not read).
-__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(from), "r"(there ? 16u : 0u) : "memory");
+// 16 bytes to shared memory, zeros behind the first `bytes` of them (which alone are read).
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 
 // Bounded wait for completion number `use` (0, 1, ..) of an mbarrier; false if it, or any
@@ -154,6 +153,7 @@ __device__ __forceinline__ void fetch_role(const Params &p, const DecodeSideDev 
     int ahead = page_of(c.first);
     uint32_t from_lo = 0, from_hi = 0;                      // where this lane's 16 tokens' codes are
     const __half *norms_from = norms;
+    uint32_t norm_bytes = 0;                                // of this lane's 16 tokens, those that exist
     bool good = false;
     for (int tile = c.first; tile < c.last; ++tile, ++T, raw.next()) {
       const int step = (tile - c.first) & 7;
@@ -166,6 +166,7 @@ __device__ __forceinline__ void fetch_role(const Params &p, const DecodeSideDev 
         from_lo = (uint32_t)from;
         from_hi = (uint32_t)(from >> 32);
         norms_from = good ? norms + (int64_t)page * sd.norm_page_stride + slot : norms;
+        norm_bytes = good ? 2u * (uint32_t)min(16, L - (tile * kTile + 16 * lane)) : 0u;
       }
       const uint32_t bar = (uint32_t)(side * kMostRaw + raw.at) * 8u, at = ring + (uint32_t)raw.at * kRawBytes;
       if (raw.use > 0 && !warp_wait(kRawFree + bar, raw.use - 1)) return;
@@ -174,7 +175,7 @@ __device__ __forceinline__ void fetch_role(const Params &p, const DecodeSideDev 
       for (int u = 0; u < 4; ++u) {
         const uint64_t lo = __shfl_sync(kFull, from_lo, 4 * step + u), hi = __shfl_sync(kFull, from_hi, 4 * step + u);
         const uint8_t *from = (const uint8_t *)(lo | hi << 32);
-        const bool there = (goods >> u & 1u) != 0;
+        const uint32_t there = (goods >> u & 1u) << 4;      // bytes of a copy
 #pragma unroll
         for (int e = 0; e < kBytes; e += 512)
           if (kBytes - e >= 512 || 16 * lane < kBytes - e)
@@ -182,14 +183,10 @@ __device__ __forceinline__ void fetch_role(const Params &p, const DecodeSideDev 
       }
       if (lane >> 2 == step) {                              // the lane that knows the page
         const uint32_t to = at + 4 * kBytes + 32u * (lane & 3);
-        copy16(to, norms_from, good);
-        copy16(to + 16, norms_from + (good ? 8 : 0), good);
+        copy16(to, norms_from, min(norm_bytes, 16u));
+        copy16(to + 16, norms_from + (good ? 8 : 0), norm_bytes > 16u ? norm_bytes - 16u : 0u);
       }
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(kRawFull + bar) : "memory");
-      if (lane == 0) {
-        sts32(kValid + 4u * (uint32_t)(side * kMostRaw + raw.at), (uint32_t)min(kTile, L - tile * kTile));
-        mbar_arrive(kRawFull + bar);
-      }
     }
   }
 }
@@ -214,13 +211,12 @@ __device__ __forceinline__ void decode_role(int tiles, int side, int u, uint32_t
     // (looked at now, waited for only when the lookups are done)
     const bool is_free = buf.use == 0 || mbar_try(tile_bar + kFreeTile + 8u * buf.at, (uint32_t)(buf.use - 1) & 1u);
     const uint32_t off = (uint32_t)raw.at * kRawBytes;
-    const uint32_t valid = lds32(kValid + 4u * (uint32_t)(side * kMostRaw + raw.at));
     uint32_t w[2][kRowBytes / 16];
     __half2 n[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       load_words<kRowBytes / 4>(codes + off + (uint32_t)(8 * h * kRowBytes), w[h]);
-      n[h] = __float2half2_rn(row + 8u * h < valid ? lds_half(norms + off + 16u * h) : 0.f);
+      n[h] = __float2half2_rn(lds_half(norms + off + 16u * h));
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -243,41 +239,64 @@ __device__ __forceinline__ void decode_role(int tiles, int side, int u, uint32_t
   }
 }
 
-// fp32 scores of this thread's query row (null: zeros) with the sixteen tokens from `tok` on, from
-// the packed codes, the same address for the whole warp.  Out of line: only for tiles whose scores
-// came out large.
+// The row's mask words of query row `qr` of a piece's kv head.
+__device__ __forceinline__ const int32_t *words_of(const Params &p, const Piece &c, int qr) {
+  return p.mask + c.b * p.mask_b + (int64_t)(qr / p.n_rep) * p.mask_t;
+}
+
+// Bits of the 64 tokens from `tok0` on that query row `qr` sees.
+__device__ __noinline__ uint2 seen_tokens(const Params &p, int b, int qr, int at) {
+  const int32_t *words = p.mask + b * p.mask_b + (int64_t)(qr / p.n_rep) * p.mask_t;
+  return make_uint2(visible(words, p.Q, at), visible(words, p.Q, at + 32));
+}
+
+// fp32 scores of query row `qr` (negative: zeros) with the 64 tokens from `tok0` on, from the packed codes,
+// the same addresses for the whole warp: the maximum over those it sees, and the half `hf` of them to `own`.
+// Out of line: only for tiles whose scores came out large.
 template <int BW, int D>
-__device__ __noinline__ void precise_scores(const uint8_t *pages, int64_t page_stride, const __half *norms,
-                                            int64_t norm_page_stride, const float *centroids, const int32_t *table, int P,
-                                            int S, int tok, int end, const float *q, float *out) {
+__device__ __noinline__ float precise_scores(const Params &p, Piece c, int qr, int tok0, int hf, uint2 seen, float *own) {
   constexpr int kRowBytes = D * BW / 8;
-  const int page = tok < end ? table[tok / S] : -1;
-  float acc[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-  if ((uint32_t)page < (uint32_t)P) {
-    const uint8_t *row = pages + (int64_t)page * page_stride + (int64_t)(tok % S) * kRowBytes;
+  const int end = length_of(p, c.b), i = qr / p.n_rep;
+  const float *q = qr < 0 ? nullptr : p.q_rot + (((int64_t)c.b * p.Q + i) * p.Hq + c.h * p.n_rep + qr - i * p.n_rep) * D;
+  float mx = -INFINITY;
 #pragma unroll 1
-    for (int d = 0; d < D / 4; ++d) {                          // four coordinates: BW / 2 bytes of each row
-      const float4 x = q ? __ldg(reinterpret_cast<const float4 *>(q) + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int blk = 0; blk < kTile / 16; ++blk) {                 // sixteen tokens of one page
+    const int tok = tok0 + 16 * blk;
+    const int page = tok < end ? p.page_table[(int64_t)c.b * p.table_stride + tok / p.S] : -1;
+    float acc[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        uint32_t w = 0;
+    for (int k = 0; k < 16; ++k) acc[k] = 0.f;
+    if ((uint32_t)page < (uint32_t)p.P) {
+      const uint8_t *row = p.k.pages + (int64_t)c.h * p.k.head_stride + (int64_t)page * p.k.page_stride +
+                           (int64_t)(tok % p.S) * kRowBytes;
+#pragma unroll 1
+      for (int d = 0; d < D / 4; ++d) {                        // four coordinates: BW / 2 bytes of each row
+        const float4 x = q ? __ldg(reinterpret_cast<const float4 *>(q) + d) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int b = 0; b < BW / 2; ++b) w |= (uint32_t)__ldg(row + i * kRowBytes + d * (BW / 2) + b) << (8 * b);
-        constexpr uint32_t kMask = (1u << BW) - 1u;
-        acc[i] = fmaf(x.x, __ldg(centroids + (w & kMask)), acc[i]);
-        acc[i] = fmaf(x.y, __ldg(centroids + ((w >> BW) & kMask)), acc[i]);
-        acc[i] = fmaf(x.z, __ldg(centroids + ((w >> (2 * BW)) & kMask)), acc[i]);
-        acc[i] = fmaf(x.w, __ldg(centroids + ((w >> (3 * BW)) & kMask)), acc[i]);
+        for (int k = 0; k < 16; ++k) {
+          uint32_t w = 0;
+#pragma unroll
+          for (int e = 0; e < BW / 2; ++e) w |= (uint32_t)__ldg(row + k * kRowBytes + d * (BW / 2) + e) << (8 * e);
+          constexpr uint32_t kMask = (1u << BW) - 1u;
+          acc[k] = fmaf(x.x, __ldg(p.k.centroids + (w & kMask)), acc[k]);
+          acc[k] = fmaf(x.y, __ldg(p.k.centroids + ((w >> BW) & kMask)), acc[k]);
+          acc[k] = fmaf(x.z, __ldg(p.k.centroids + ((w >> (2 * BW)) & kMask)), acc[k]);
+          acc[k] = fmaf(x.w, __ldg(p.k.centroids + ((w >> (3 * BW)) & kMask)), acc[k]);
+        }
       }
+      const __half *nrm = p.k.norms + (int64_t)c.h * p.k.norm_head_stride + (int64_t)page * p.k.norm_page_stride + tok % p.S;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) acc[k] *= tok + k < end ? __half2float(nrm[k]) : 0.f;
     }
-    const __half *nrm = norms + (int64_t)page * norm_page_stride + tok % S;
+    const uint32_t bits = (blk < 2 ? seen.x : seen.y) >> (16 * (blk & 1));
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] *= tok + i < end ? __half2float(nrm[i]) : 0.f;
+    for (int k = 0; k < 16; ++k) {
+      const float v = (bits >> k & 1u) ? acc[k] : -INFINITY;
+      mx = fmaxf(mx, v);
+      if (blk >> 1 == hf) own[16 * (blk & 1) + k] = v;
+    }
   }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) out[i] = acc[i];
+  return mx;
 }
 
 // Scores of unseen tokens become -inf (`seen`: a bit per token).
@@ -296,7 +315,7 @@ __device__ __forceinline__ float maximum(const uint32_t (&s)[32]) {
 }
 
 template <int BWK, int BWV, int D>
-__global__ void __launch_bounds__(kThreads, 1) scan_kernel(Params p) {
+__global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant__ Params p) {
   using M = Map<BWK, BWV, D>;
   extern __shared__ __align__(128) uint8_t dyn_smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -321,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(Params p) {
     }
 #pragma unroll
     for (int i = 0; i < 2 * kMostRaw; ++i) {
-      mbar_init(kRawFull + 8u * i, 33);                     // 32 lanes' copies, and the word beside them
+      mbar_init(kRawFull + 8u * i, 32);                     // every lane's copies
       mbar_init(kRawFree + 8u * i, 4);
     }
 #pragma unroll
@@ -362,13 +381,14 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(Params p) {
       const int nt = c.last - c.first;
       x += nt;
       const int L = length_of(p, c.b), hist = L - p.Q, qr = c.rb * kRows + r;
-      const int i = qr / p.n_rep;
-      const int32_t *words = p.mask + c.b * p.mask_b + i * p.mask_t;
-      const bool live = qr < p.R && !padding(words, p.Q);
+      const bool live = qr < p.R && !padding(words_of(p, c, qr), p.Q);
       const bool working = __any_sync(kFull, live);         // a warp without live rows only keeps step
-      const int64_t row = ((int64_t)c.b * p.Q + i) * p.Hq + c.h * p.n_rep + qr - i * p.n_rep;
-      const float *q = live ? p.q_rot + row * D : nullptr;
+      auto row_of = [&]() -> int64_t {                      // of the (B, Q, Hq) states
+        const int i = qr / p.n_rep;
+        return ((int64_t)c.b * p.Q + i) * p.Hq + c.h * p.n_rep + qr - i * p.n_rep;
+      };
       {
+        const float *q = live ? p.q_rot + row_of() * D : nullptr;
         // this warpgroup's quarter of the query rows into tensor memory (the products of the last piece are done)
         constexpr int kPart = D / 4;
         const int part = warp >> 2;
@@ -403,41 +423,25 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(Params p) {
         tmem_load32<0>(s_addr + 32u * (hf ^ 1), s);         // the other half, for its maximum
         tmem_wait_load();
         const bool masked = tok0 + kTile > hist;
-        uint32_t seen = kFull, seen_other = kFull;
-        if (masked && live) {
-          seen = visible(words, p.Q, tok0 + 32 * hf - hist);
-          seen_other = visible(words, p.Q, tok0 + 32 * (hf ^ 1) - hist);
-        }
-        if (masked) hide(s, seen_other);
+        uint2 seen = make_uint2(kFull, kFull);
+        if (masked && live) seen = seen_tokens(p, c.b, qr, tok0 - hist);
+        if (masked) hide(s, hf ? seen.x : seen.y);
         float mx = maximum(s);
         tmem_load32<0>(s_addr + 32u * hf, s);
         tmem_wait_load();
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(kSFree + 8u * st);       // the scores are in registers
-        if (masked) hide(s, seen);
+        if (masked) hide(s, hf ? seen.y : seen.x);
         mx = fmaxf(mx, maximum(s));
         const bool large = !(fabsf(mx) <= kPreciseAbove) && mx != -INFINITY;
         bool drained = k == 0;                              // the stream's last products have ended
         if (__any_sync(kFull, large || mx > ref + kSlack || (ref == -INFINITY && mx != -INFINITY))) {
           if (__any_sync(kFull, large)) {
-            const int32_t *table = p.page_table + (int64_t)c.b * p.table_stride;
-            float t16[16];
-            mx = -INFINITY;
+            float own[32];
+            mx = precise_scores<BWK, D>(p, c, live ? qr : -1, tok0, hf, seen, own);
 #pragma unroll
-            for (int blk = 0; blk < 4; ++blk) {             // the other half's tokens, then the own ones
-              const int half = blk < 2 ? hf ^ 1 : hf, tok = tok0 + 32 * half + 16 * (blk & 1);
-              precise_scores<BWK, D>(p.k.pages + (int64_t)c.h * p.k.head_stride, p.k.page_stride,
-                                     p.k.norms + (int64_t)c.h * p.k.norm_head_stride, p.k.norm_page_stride, p.k.centroids,
-                                     table, p.P, p.S, tok, L, q, t16);
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const int bit = 16 * (blk & 1) + e;
-                const float v = ((blk < 2 ? seen_other : seen) >> bit & 1u) ? t16[e] : -INFINITY;
-                mx = fmaxf(mx, v);
-                if (blk >= 2) s[bit] = __float_as_uint(v);
-              }
-            }
+            for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(own[e]);
           }
           const float now = mx > ref + kSlack || ref == -INFINITY ? mx : ref;
           if (k > 0 && __any_sync(kFull, now != ref)) {     // rescale what is accumulated
@@ -495,6 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(Params p) {
         const float w0 = m0 == -INFINITY ? 0.f : ex2(m0 - top), w1 = m1 == -INFINITY ? 0.f : ex2(m1 - top);
         const float total = w0 * (state(1) + state(2)) + w1 * (state(4) + state(5));
         float *acc;
+        const int64_t row = row_of();
         if (c.slot < 0) {
           acc = p.acc + row * D;
           if (warp < 4 && qr < p.R) p.m[row] = live ? top : -INFINITY, p.l[row] = live ? total : 0.f;
