@@ -4,24 +4,24 @@
 // The query rows of a group lie in tensor memory as the fp16 A operand of all score products.  The
 // group's tiles alternate between two streams, each with scores, probabilities, accumulator, running
 // maximum and sum of its own, so that one stream's softmax runs under the other's products; the two
-// states are joined when the piece ends.  Twenty-eight warps in roles that meet at mbarriers only:
+// states are joined when the piece ends.  Twenty to twenty-eight warps in roles that meet at mbarriers only:
 //
 //   fetch     a warp per side: codes and norms of a tile into a ring of raw tiles, 16 bytes a copy;
-//   decode    four warps per side, one for every 16 tokens of a tile: codes through the per-lane lookup
-//             tables (wtq_lut.cuh) to fp16 centroid times norm in the canonical operand layout, three
-//             tiles deep;
+//   decode    four or eight warps per side, one for every 16 or 8 tokens of a tile: codes through the
+//             per-lane lookup tables (wtq_lut.cuh) to fp16 centroid times norm in the canonical operand
+//             layout, three tiles deep;
 //   multiply  a warp for S = Q K^T (N 64) and one for O += P V (A = P from tensor memory, V read with
 //             tokens as the contraction), an elected lane of each issues;
-//   softmax   two warpgroups per stream, a thread per query row and half of a tile's tokens: both take
-//             the maximum over the whole tile, which costs less than exchanging it, and the
-//             exponentials of their own half.  O is rescaled only when a row's maximum grows by 2^8.
+//   softmax   a warpgroup per stream, a thread per query row: scores from tensor memory, handed back at
+//             once; tree mask, running maximum, probabilities as fp16.  O is rescaled only when a row's
+//             maximum grows by 2^8.
 //
 // The roles walk the static schedule by themselves: fetch and decode work into the next piece while
 // the softmax warps write the last one's states.  Every wait is bounded; one that runs out raises a
 // flag that ends all others, and the status word says so.
 //
 // A warp on its own gets through an instruction in about nine cycles here, so a role is only as fast
-// as its instructions per tile are few: the split above gives every warp 100 to 150 of them.
+// as its instructions per tile are few.
 //
 // fp16 scores carry an error that grows with |q| |k|; a warp whose tile holds a row maximum beyond
 // kPreciseAbove (log2 domain) recomputes that tile's scores in fp32 from the packed codes.
@@ -40,8 +40,10 @@ namespace um {
 
 using namespace umma;
 
-constexpr int kSoftWarps = 16, kDecodeWarp = kSoftWarps, kFetchWarp = kDecodeWarp + 8;
-constexpr int kScoreWarp = kFetchWarp + 2, kValueWarp = kScoreWarp + 1, kThreads = 32 * (kValueWarp + 1);
+constexpr int kSoftWarps = 8;
+// Decode warps of a side: a code of 6 or 8 bits takes a lookup of its own and twice the instructions of
+// a 4-bit one, so those sides have a warp for every 8 tokens of a tile instead of 16.
+__host__ __device__ constexpr int decode_warps(int bw) { return bw == 4 ? 4 : 8; }
 constexpr int kRows = kUmmaRows, kTile = kUmmaTile;
 constexpr int kStages = 3;                      // decoded tiles of a side
 constexpr int kMostRaw = 5;                     // raw tiles of a side: as many of these as fit
@@ -54,9 +56,9 @@ constexpr uint32_t kSFull = kRawFree + 16 * kMostRaw, kSFree = kSFull + 16, kPFu
                    kODone = kPFull + 16;                                   // [stream]
 constexpr uint32_t kQFull = kODone + 16, kLast = kQFull + 8, kTmemSlot = kLast + 8, kAbort = kTmemSlot + 4;
 constexpr uint32_t kPrefix = kBase + 512;                                  // kMaxBatch + 1 words
-constexpr uint32_t kStates = kPrefix + 4 * (kMaxBatch + 4);                // [stream][m, l of a half, l of the other][row]
+constexpr uint32_t kStates = kPrefix + 4 * (kMaxBatch + 4);                // [stream][m, l][row]
 constexpr uint32_t kVTile = 16384;
-static_assert(kAbort + 4 <= kPrefix && kStates + 6 * kRows * 4 <= kVTile, "low region");
+static_assert(kAbort + 4 <= kPrefix && kStates + 4 * kRows * 4 <= kVTile, "low region");
 static_assert(kVTile + kStages * kTile * 256 <= mma::kLutAddr, "value tiles end where the tables begin");
 // tensor memory columns
 constexpr uint32_t kColQ = 0, kColS = 64, kColP = 192, kColO = 256, kCols = 512;   // S + 64, P + 32, O + 128 per stream
@@ -67,6 +69,8 @@ constexpr int kWaitTries = 1 << 20;
 template <int BWK, int BWV, int D> struct Map {
   static constexpr int kEntries = mma::lut_entries(BWK) > mma::lut_entries(BWV) ? mma::lut_entries(BWK)
                                                                                 : mma::lut_entries(BWV);
+  static constexpr int kDecodeK = kSoftWarps, kDecodeV = kDecodeK + decode_warps(BWK), kFetch = kDecodeV + decode_warps(BWV);
+  static constexpr int kScore = kFetch + 2, kValue = kScore + 1, kThreads = 32 * (kValue + 1);
   static constexpr uint32_t kGroup = (uint32_t)D * 16u;                    // eight rows of an operand tile
   static constexpr uint32_t kTileBytes = kTile / 8 * kGroup;
   static constexpr uint32_t kKTile = mma::kLutAddr + (uint32_t)kEntries * 256u;
@@ -191,17 +195,18 @@ __device__ __forceinline__ void fetch_role(const Params &p, const DecodeSideDev 
   }
 }
 
-// One decode warp: tokens 16 u .. 16 u + 15 of every tile of a side, lane (g, t) rows g and g + 8,
-// coordinates t * D / 4 on.
+// One decode warp: its eight or sixteen tokens of every tile of a side, lane (g, t) rows g (and g + 8) of
+// them, coordinates t * D / 4 on.
 template <int BW, int D, int RAW_TILES>
 __device__ __forceinline__ void decode_role(int tiles, int side, int u, uint32_t ring, uint32_t tile_base) {
   constexpr int kRowBytes = D * BW / 8, kPairs = D / 8;     // code pairs of a quarter
+  constexpr int kGroups = 8 / decode_warps(BW);             // groups of eight tokens
   constexpr uint32_t kRawBytes = kTile * kRowBytes + 2 * kTile, kTileBytes = kTile * D * 2;
   const int lane = threadIdx.x & 31, g = lane & 7, t = lane >> 3;
   const uint32_t sel = mma::kLutAddr | (uint32_t)(lane << 2) | (side ? 0x80u : 0u);
-  const uint32_t row = (uint32_t)(16 * u + g);
+  const uint32_t row = (uint32_t)(8 * kGroups * u + g);
   const uint32_t codes = ring + row * kRowBytes + (uint32_t)t * (kRowBytes / 4), norms = ring + kTile * kRowBytes + 2u * row;
-  const uint32_t to = tile_base + (uint32_t)(2 * u) * (uint32_t)(D * 16) + (uint32_t)t * (D / 32 * 128) + (uint32_t)g * 16u;
+  const uint32_t to = tile_base + (uint32_t)(kGroups * u) * (uint32_t)(D * 16) + (uint32_t)t * (D / 32 * 128) + (uint32_t)g * 16u;
   const uint32_t raw_bar = kRawFull + (uint32_t)(side * kMostRaw) * 8u, tile_bar = kTileFull + (uint32_t)(side * kStages) * 8u;
   constexpr uint32_t kFreeRaw = kRawFree - kRawFull, kFreeTile = kTileFree - kTileFull;
   Ring<RAW_TILES> raw;
@@ -211,15 +216,15 @@ __device__ __forceinline__ void decode_role(int tiles, int side, int u, uint32_t
     // (looked at now, waited for only when the lookups are done)
     const bool is_free = buf.use == 0 || mbar_try(tile_bar + kFreeTile + 8u * buf.at, (uint32_t)(buf.use - 1) & 1u);
     const uint32_t off = (uint32_t)raw.at * kRawBytes;
-    uint32_t w[2][kRowBytes / 16];
-    __half2 n[2];
+    uint32_t w[kGroups][kRowBytes / 16];
+    __half2 n[kGroups];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < kGroups; ++h) {
       load_words<kRowBytes / 4>(codes + off + (uint32_t)(8 * h * kRowBytes), w[h]);
       n[h] = __float2half2_rn(lds_half(norms + off + 16u * h));
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < kGroups; ++h) {
       uint32_t f[kPairs];
       quarter_codes<BW>(w[h], sel, f, std::make_integer_sequence<int, kPairs>{});
 #pragma unroll
@@ -251,14 +256,13 @@ __device__ __noinline__ uint2 seen_tokens(const Params &p, int b, int qr, int at
 }
 
 // fp32 scores of query row `qr` (negative: zeros) with the 64 tokens from `tok0` on, from the packed codes,
-// the same addresses for the whole warp: the maximum over those it sees, and the half `hf` of them to `own`.
+// the same addresses for the whole warp, to `own`; those it does not see are -inf.
 // Out of line: only for tiles whose scores came out large.
 template <int BW, int D>
-__device__ __noinline__ float precise_scores(const Params &p, Piece c, int qr, int tok0, int hf, uint2 seen, float *own) {
+__device__ __noinline__ void precise_scores(const Params &p, Piece c, int qr, int tok0, uint2 seen, float *own) {
   constexpr int kRowBytes = D * BW / 8;
   const int end = length_of(p, c.b), i = qr / p.n_rep;
   const float *q = qr < 0 ? nullptr : p.q_rot + (((int64_t)c.b * p.Q + i) * p.Hq + c.h * p.n_rep + qr - i * p.n_rep) * D;
-  float mx = -INFINITY;
 #pragma unroll 1
   for (int blk = 0; blk < kTile / 16; ++blk) {                 // sixteen tokens of one page
     const int tok = tok0 + 16 * blk;
@@ -290,32 +294,29 @@ __device__ __noinline__ float precise_scores(const Params &p, Piece c, int qr, i
     }
     const uint32_t bits = (blk < 2 ? seen.x : seen.y) >> (16 * (blk & 1));
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const float v = (bits >> k & 1u) ? acc[k] : -INFINITY;
-      mx = fmaxf(mx, v);
-      if (blk >> 1 == hf) own[16 * (blk & 1) + k] = v;
-    }
+    for (int k = 0; k < 16; ++k) own[16 * blk + k] = (bits >> k & 1u) ? acc[k] : -INFINITY;
   }
-  return mx;
 }
 
 // Scores of unseen tokens become -inf (`seen`: a bit per token).
-__device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t seen) {
+__device__ __forceinline__ void hide(uint32_t (&s)[64], uint2 seen) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) s[i] = (seen >> i & 1u) ? s[i] : 0xff800000u;
+  for (int i = 0; i < 64; ++i) s[i] = ((i < 32 ? seen.x >> i : seen.y >> (i - 32)) & 1u) ? s[i] : 0xff800000u;
 }
-__device__ __forceinline__ float maximum(const uint32_t (&s)[32]) {
-  float a = -INFINITY, c = -INFINITY;
+__device__ __forceinline__ float maximum(const uint32_t (&s)[64]) {
+  float a = -INFINITY, b = -INFINITY, c = -INFINITY, d = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < 32; i += 4) {
+  for (int i = 0; i < 64; i += 8) {
     a = max3(a, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-    c = max3(c, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+    b = max3(b, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+    c = max3(c, __uint_as_float(s[i + 4]), __uint_as_float(s[i + 5]));
+    d = max3(d, __uint_as_float(s[i + 6]), __uint_as_float(s[i + 7]));
   }
-  return fmaxf(a, c);
+  return fmaxf(max3(a, b, c), d);
 }
 
 template <int BWK, int BWV, int D>
-__global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(Map<BWK, BWV, D>::kThreads, 1) scan_kernel(const __grid_constant__ Params p) {
   using M = Map<BWK, BWV, D>;
   extern __shared__ __align__(128) uint8_t dyn_smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -325,9 +326,9 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant
   }
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   int *prefix = reinterpret_cast<int *>(dyn_smem + (kPrefix - (uint32_t)__cvta_generic_to_shared(dyn_smem)));
-  for (int e = tid; e < M::kEntries * 64; e += kThreads)
+  for (int e = tid; e < M::kEntries * 64; e += M::kThreads)
     sts32(mma::kLutAddr + 4u * e, mma::lut_word(e, BWK, BWV, p.k.centroids, p.v.centroids));
-  if (warp == kScoreWarp) {
+  if (warp == M::kScore) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(kTmemSlot),
                  "r"(kCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
@@ -335,19 +336,19 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant
   if (tid == 0) {
 #pragma unroll
     for (int i = 0; i < 2 * kStages; ++i) {
-      mbar_init(kTileFull + 8u * i, 4);                     // the four 16-token groups of a tile
+      mbar_init(kTileFull + 8u * i, decode_warps(i < kStages ? BWK : BWV));
       mbar_init(kTileFree + 8u * i, 1);
     }
 #pragma unroll
     for (int i = 0; i < 2 * kMostRaw; ++i) {
       mbar_init(kRawFull + 8u * i, 32);                     // every lane's copies
-      mbar_init(kRawFree + 8u * i, 4);
+      mbar_init(kRawFree + 8u * i, decode_warps(i < kMostRaw ? BWK : BWV));
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       mbar_init(kSFull + 8u * i, 1);
-      mbar_init(kSFree + 8u * i, 8);                        // the eight warps of a stream
-      mbar_init(kPFull + 8u * i, 8);
+      mbar_init(kSFree + 8u * i, 4);                        // the four warps of a stream
+      mbar_init(kPFull + 8u * i, 4);
       mbar_init(kODone + 8u * i, 1);
     }
     mbar_init(kQFull, kSoftWarps);
@@ -362,16 +363,18 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant
   const long long share = run_length(p, prefix), all = (long long)prefix[p.B] * p.row_blocks * p.Hkv;
   const long long begin = share * blockIdx.x, end = min(all, begin + share);
 
-  // Registers go from the other warps to the softmax warps: 512 x 88 + 384 x 48 of the 896 x 72 that
-  // the block was launched with.
-  if (warp < kSoftWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 88;\n");
-  else asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");
+  // Registers go from the other warps to the softmax warps, which hold 64 scores a thread: of the 640 x 96,
+  // 768 x 80 or 896 x 72 that the block was launched with, 256 x 144 and 384 x 64, 512 x 48 or 640 x 40.
+  if (warp < kSoftWarps) asm volatile("setmaxnreg.inc.sync.aligned.u32 144;\n");
+  else if constexpr (M::kThreads == 640) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n");
+  else if constexpr (M::kThreads == 768) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 40;\n");
 
   if (warp < kSoftWarps) {
-    // ================= softmax: stream `st`, tokens 32 hf .. of its tiles, one query row per thread ======
-    const int st = warp >> 3, hf = (warp >> 2) & 1, r = 32 * (warp & 3) + lane;
+    // ================= softmax: stream `st`, one query row per thread =======================
+    const int st = warp >> 2, r = 32 * (warp & 3) + lane;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t s_addr = tmem + lanes + kColS + 64u * st, p_addr = tmem + lanes + kColP + 32u * st + 16u * hf,
+    const uint32_t s_addr = tmem + lanes + kColS + 64u * st, p_addr = tmem + lanes + kColP + 32u * st,
                    o_addr = tmem + lanes + kColO + 128u * st;
     int n = 0;                                              // units of this stream so far
     bool ok = true;
@@ -388,20 +391,19 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant
         return ((int64_t)c.b * p.Q + i) * p.Hq + c.h * p.n_rep + qr - i * p.n_rep;
       };
       {
+        // this warpgroup's half of the query rows into tensor memory (the products of the last piece are done)
         const float *q = live ? p.q_rot + row_of() * D : nullptr;
-        // this warpgroup's quarter of the query rows into tensor memory (the products of the last piece are done)
-        constexpr int kPart = D / 4;
-        const int part = warp >> 2;
+        constexpr int kPart = D / 2;
         uint32_t v[kPart / 2];
 #pragma unroll
         for (int k = 0; k < kPart / 4; ++k) {
-          const float4 y = q ? __ldg(reinterpret_cast<const float4 *>(q + kPart * part) + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float4 y = q ? __ldg(reinterpret_cast<const float4 *>(q + kPart * st) + k) : make_float4(0.f, 0.f, 0.f, 0.f);
           v[2 * k] = pack_half2(y.x, y.y);
           v[2 * k + 1] = pack_half2(y.z, y.w);
         }
-        const uint32_t to = tmem + lanes + kColQ + (uint32_t)(kPart / 2 * part);
-        if constexpr (D == 128) tmem_store16(to, v);
-        else tmem_store8(to, v);
+        const uint32_t to = tmem + lanes + kColQ + (uint32_t)(kPart / 2 * st);
+        if constexpr (D == 128) tmem_store32(to, v);
+        else tmem_store16(to, v);
       }
       tmem_wait_store();
       fence_before();
@@ -419,29 +421,29 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant
           continue;
         }
         fence_after();
-        uint32_t s[32];
-        tmem_load32<0>(s_addr + 32u * (hf ^ 1), s);         // the other half, for its maximum
-        tmem_wait_load();
-        const bool masked = tok0 + kTile > hist;
-        uint2 seen = make_uint2(kFull, kFull);
-        if (masked && live) seen = seen_tokens(p, c.b, qr, tok0 - hist);
-        if (masked) hide(s, hf ? seen.x : seen.y);
-        float mx = maximum(s);
-        tmem_load32<0>(s_addr + 32u * hf, s);
+        uint32_t s[64];
+        tmem_load32<0>(s_addr, s);
+        tmem_load32<32>(s_addr + 32, s);
         tmem_wait_load();
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(kSFree + 8u * st);       // the scores are in registers
-        if (masked) hide(s, hf ? seen.y : seen.x);
-        mx = fmaxf(mx, maximum(s));
+        const bool masked = tok0 + kTile > hist;
+        uint2 seen = make_uint2(kFull, kFull);
+        if (masked) {
+          if (live) seen = seen_tokens(p, c.b, qr, tok0 - hist);
+          hide(s, seen);
+        }
+        float mx = maximum(s);
         const bool large = !(fabsf(mx) <= kPreciseAbove) && mx != -INFINITY;
         bool drained = k == 0;                              // the stream's last products have ended
         if (__any_sync(kFull, large || mx > ref + kSlack || (ref == -INFINITY && mx != -INFINITY))) {
           if (__any_sync(kFull, large)) {
-            float own[32];
-            mx = precise_scores<BWK, D>(p, c, live ? qr : -1, tok0, hf, seen, own);
+            float own[64];
+            precise_scores<BWK, D>(p, c, live ? qr : -1, tok0, seen, own);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(own[e]);
+            for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(own[e]);
+            mx = maximum(s);
           }
           const float now = mx > ref + kSlack || ref == -INFINITY ? mx : ref;
           if (k > 0 && __any_sync(kFull, now != ref)) {     // rescale what is accumulated
@@ -451,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant
             const float scale = ref == now ? 1.f : ref == -INFINITY ? 0.f : ex2(ref - now);
             sum *= scale;
 #pragma unroll 1
-            for (int c0 = hf * (D / 2); c0 < (hf + 1) * (D / 2); c0 += 16) {
+            for (int c0 = 0; c0 < D; c0 += 16) {
               uint32_t o[16];
               tmem_load16(o_addr + c0, o);
               tmem_wait_load();
@@ -464,78 +466,76 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant
           ref = now;
         }
         const uint64_t base = twice(ref == -INFINITY ? 0.f : -ref);
-        uint32_t pr[16];
-        uint64_t sums = 0;                                  // (the bits of two zeros)
+        uint32_t pr[32];
+        uint64_t sums[2] = {0, 0};                          // (the bits of two zeros)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < 32; ++e) {
           const float2 y = halves(add2(pair(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), base));
           const float a = ex2(y.x), b = ex2(y.y);
-          sums = add2(sums, pair(a, b));
+          sums[e & 1] = add2(sums[e & 1], pair(a, b));
           pr[e] = pack_half2(a, b);
         }
-        const float2 both = halves(sums);
+        const float2 both = halves(add2(sums[0], sums[1]));
         sum += both.x + both.y;
         if (!drained) {                                     // the last products have read their probabilities
           if (!(ok = warp_wait(kODone + 8u * st, n - 1))) break;
           fence_after();
         }
-        tmem_store16(p_addr, pr);
+        tmem_store32(p_addr, pr);
         tmem_wait_store();
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(kPFull + 8u * st);
       }
-      // ---- the rows' states: the two streams joined, a quarter of the coordinates to each warpgroup ----
+      // ---- the rows' states: the two streams joined, half of the coordinates to each warpgroup ----
       if (ok && mine > 0) ok = warp_wait(kODone + 8u * st, n - 1);
-      if (hf == 0) sts32(kStates + 4u * ((3 * st) * kRows + r), __float_as_uint(ref));
-      sts32(kStates + 4u * ((3 * st + 1 + hf) * kRows + r), __float_as_uint(sum));
+      sts32(kStates + 4u * ((2 * st) * kRows + r), __float_as_uint(ref));
+      sts32(kStates + 4u * ((2 * st + 1) * kRows + r), __float_as_uint(sum));
       fence_before();
       asm volatile("bar.sync 1, %0;\n" ::"r"(32 * kSoftWarps) : "memory");   // every softmax warp, whatever it gave up on
       fence_after();
       ok = __all_sync(kFull, ok && lds32(kAbort) == 0u);
       if (ok) {
         auto state = [&](int what) { return __uint_as_float(lds32(kStates + 4u * (what * kRows + r))); };
-        const float m0 = state(0), m1 = state(3), top = fmaxf(m0, m1);
+        const float m0 = state(0), m1 = state(2), top = fmaxf(m0, m1);
         const float w0 = m0 == -INFINITY ? 0.f : ex2(m0 - top), w1 = m1 == -INFINITY ? 0.f : ex2(m1 - top);
-        const float total = w0 * (state(1) + state(2)) + w1 * (state(4) + state(5));
+        const float total = w0 * state(1) + w1 * state(3);
         float *acc;
         const int64_t row = row_of();
         if (c.slot < 0) {
           acc = p.acc + row * D;
-          if (warp < 4 && qr < p.R) p.m[row] = live ? top : -INFINITY, p.l[row] = live ? total : 0.f;
+          if (st == 0 && qr < p.R) p.m[row] = live ? top : -INFINITY, p.l[row] = live ? total : 0.f;
         } else {
           const int64_t at = ((int64_t)blockIdx.x * 2 + c.slot) * kRows + r;
           acc = p.part_acc + at * D;
-          if (warp < 4) p.part_m[at] = live ? top : -INFINITY, p.part_l[at] = live ? total : 0.f;
+          if (st == 0) p.part_m[at] = live ? top : -INFINITY, p.part_l[at] = live ? total : 0.f;
         }
-        constexpr int kPart = D / 4;
-        const int part = warp >> 2;
 #pragma unroll 1
-        for (int c0 = kPart * part; c0 < kPart * (part + 1); c0 += 16) {
-          uint32_t o[16], o1[16];
-          tmem_load16(tmem + lanes + kColO + c0, o);
-          if (nt > 1) tmem_load16(tmem + lanes + kColO + 128 + c0, o1);
+        for (int c0 = st * (D / 2); c0 < (st + 1) * (D / 2); c0 += 32) {
+          uint32_t o[32], o1[32];
+          tmem_load32<0>(tmem + lanes + kColO + c0, o);
+          if (nt > 1) tmem_load32<0>(tmem + lanes + kColO + 128 + c0, o1);
           tmem_wait_load();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
+          for (int e = 0; e < 32; ++e) {
             float v = __uint_as_float(o[e]) * w0;
             if (nt > 1) v = fmaf(__uint_as_float(o1[e]), w1, v);
             o[e] = __float_as_uint(v);
           }
           if (live) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < 8; ++e)
               reinterpret_cast<uint4 *>(acc + c0)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
         }
       }
     }
-  } else if (warp < kFetchWarp) {
-    const int side = (warp - kDecodeWarp) >> 2, tiles = (int)max(0LL, end - begin);
-    if (side == 0) decode_role<BWK, D, M::kRawTiles>(tiles, 0, warp & 3, M::kRaw, M::kKTile);
-    else decode_role<BWV, D, M::kRawTiles>(tiles, 1, warp & 3, M::kRaw + M::kRawTiles * M::kRawK, kVTile);
-  } else if (warp < kScoreWarp) {
-    if (warp == kFetchWarp) fetch_role<BWK, D, M::kRawTiles>(p, p.k, prefix, begin, end, 0, M::kRaw);
+  } else if (warp < M::kFetch) {
+    const int tiles = (int)max(0LL, end - begin);
+    if (warp < M::kDecodeV) decode_role<BWK, D, M::kRawTiles>(tiles, 0, warp - M::kDecodeK, M::kRaw, M::kKTile);
+    else decode_role<BWV, D, M::kRawTiles>(tiles, 1, warp - M::kDecodeV, M::kRaw + M::kRawTiles * M::kRawK, kVTile);
+  } else if (warp < M::kScore) {
+    if (warp == M::kFetch) fetch_role<BWK, D, M::kRawTiles>(p, p.k, prefix, begin, end, 0, M::kRaw);
     else fetch_role<BWV, D, M::kRawTiles>(p, p.v, prefix, begin, end, 1, M::kRaw + M::kRawTiles * M::kRawK);
     asm volatile("cp.async.wait_all;\n" ::: "memory");     // (a block that gave up leaves no copies behind)
   } else {
@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant
       const Piece c = piece_at(p, prefix, x, begin, end);
       const int nt = c.last - c.first;
       x += nt;
-      if (warp == kScoreWarp) {
+      if (warp == M::kScore) {
         ok = warp_wait(kQFull, pieces);
         fence_after();
         for (int j = 0; j < nt && ok; ++j, buf.next()) {    // S of the piece's tile j
@@ -591,12 +591,12 @@ __global__ void __launch_bounds__(kThreads, 1) scan_kernel(const __grid_constant
   if (tid == 0 && lds32(kAbort) != 0u && p.status) atomicOr(p.status, WTQ_STATUS_SCAN_TIMEOUT);
   // A block that gave up may have products in flight: they end before their tensor memory
   // goes to somebody else (bounded, like every wait).  Each of the two warps answers for its own.
-  if (warp >= kScoreWarp) {
+  if (warp >= M::kScore) {
     fence_after();
     if (elect_one()) umma_commit(kLast);
     __syncwarp();
   }
-  if (warp == kScoreWarp) {
+  if (warp == M::kScore) {
     for (int spin = 0; spin < kWaitTries && !mbar_try(kLast, 0u); ++spin) {
     }
     __syncwarp();
@@ -615,7 +615,7 @@ template <int BWK, int BWV, int D> int launch(const Params &p, cudaStream_t stre
     if (e != cudaSuccess) return check_cuda(e, "wtq_tree: shared memory opt-in");
     opted_in[dev & 63].store(true, std::memory_order_release);
   }
-  return launch_behind(scan_kernel<BWK, BWV, D>, p.blocks, kThreads, M::kDynamic, stream, "wtq_tree scan launch", p);
+  return launch_behind(scan_kernel<BWK, BWV, D>, p.blocks, M::kThreads, M::kDynamic, stream, "wtq_tree scan launch", p);
 }
 template <int D> int launch_widths(const Params &p, cudaStream_t stream) {
   if (p.k.bw == 4 && p.v.bw == 4) return launch<4, 4, D>(p, stream);
