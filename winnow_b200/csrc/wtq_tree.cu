@@ -248,6 +248,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(Params p) {
         for (int d = tid & 3; d < padded; d += 4) qs[r * pitch + d] = qr < p.R && d < p.D ? from[d] : 0.f;
       }
     }
+    const bool idle = row0 + 8 * warp >= p.R;             // a warp whose rows do not exist
     float m[8], l[8];                                     // of rows 8 warp .. 8 warp + 7
     bool dead[8];
 #pragma unroll
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(Params p) {
       decode_rows(p, table, c.h, tok0, L, cents, ks, vs, pitch, padded);
       __syncthreads();
       float s[4][2] = {};
-      for (int d = 0; d < padded; d += 4) {
+      for (int d = 0; d < (idle ? 0 : padded); d += 4) {
         float4 q4[4], k4[2];
 #pragma unroll
         for (int r = 0; r < 4; ++r) q4[r] = *reinterpret_cast<const float4 *>(qs + (4 * ty + r) * pitch + d);
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(Params p) {
 #pragma unroll
         for (int j = 0; j < 4 * NJ; ++j) acc[r][j] *= f;
       }
-      for (int t0 = 0; t0 < kScanTile; t0 += 4) {
+      for (int t0 = 0; t0 < (idle ? 0 : kScanTile); t0 += 4) {
         float4 w4[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) w4[r] = *reinterpret_cast<const float4 *>(ps + (4 * ty + r) * kP + t0);
@@ -452,7 +453,7 @@ extern "C" int wtq_tree(const void *q, int dtype, const int64_t q_strides[3], vo
   p.tile = umma ? tree::kUmmaTile : tree::kScanTile;
   p.row_blocks = (p.R + p.rows - 1) / p.rows;
   p.blocks = tree::scan_blocks(umma, D);
-  p.least = 2;
+  p.least = umma ? 2 : 1;
   const int el = dtype == WTQ_F32 ? 4 : 2;
   for (int b0 = 0; b0 < B; b0 += tree::kMaxBatch) {
     p.B = std::min(B - b0, tree::kMaxBatch);

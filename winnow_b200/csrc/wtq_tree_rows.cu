@@ -2,9 +2,10 @@
 // queries into the key basis (q_rot = q_scale * q Pi_K^T) and joined states out of the value basis
 // (out = a Pi_V, a = sum_c w_c acc_c / sum_c w_c l_c).
 //
-// 128 rows a block, one accumulator.  Both factors are split into fp16 high and low parts and three
+// Up to 128 rows a block, one accumulator.  Both factors are split into fp16 high and low parts and three
 // products summed in fp32, which leaves 2^-22 of the result as error, the class of an fp32 product
-// (16-bit queries have no low part: two products).  A row is scaled by a power of two to its largest
+// (16-bit queries have no low part: two products; neither do states that leave as bf16, whose rounding is
+// eight times that of the fp16 high part).  A row is scaled by a power of two to its largest
 // element first, and Pi by 2^8, so that low parts stay clear of fp16's subnormal range.  Pi is laid out
 // as the operand once and serves both: read along its rows for the queries (K-major), across them for
 // the states (MN-major).  A thread per row quarter converts and stores.  Bound by the reads of rows and of
@@ -27,11 +28,12 @@ constexpr float kPiScale = 256.f;
 
 template <int D> struct Map {
   static constexpr uint32_t kGroup = (uint32_t)D * 16u;     // eight rows of an operand
-  static constexpr uint32_t kA = 1024, kABytes = kRows / 8 * kGroup;
-  static constexpr uint32_t kB = kA + 2 * kABytes, kBBytes = D / 8 * kGroup;
-  static constexpr uint32_t kScales = kB + 2 * kBBytes;     // a row's power of two
+  static constexpr uint32_t kScales = 1024;                 // a row's power of two
   static constexpr uint32_t kBar = kScales + 4 * kRows, kSlot = kBar + 8, kPrefix = kSlot + 8;
-  static constexpr uint32_t kBytes = kPrefix + 4 * (kMaxBatch + 1);
+  static constexpr uint32_t kA = 10240, kABytes = kRows / 8 * kGroup, kBBytes = D / 8 * kGroup;
+  static constexpr uint32_t kB = kA + kABytes, kALow = kB + 2 * kBBytes;     // the rows' low parts, where there are any
+  static constexpr uint32_t kBytes = kALow + kABytes;
+  static_assert(kPrefix + 4 * (kMaxBatch + 1) <= kA, "low region");
   static constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
 };
 
@@ -39,7 +41,7 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t *>(&h);
 }
-// Eight values as fp16 high parts at `at`, what they leave as low parts at `at` + `low`.
+// Eight values as fp16 high parts at `at`, what they leave as low parts at `at` + `low` (0: dropped).
 __device__ __forceinline__ void store_split(uint32_t at, uint32_t low, const float (&x)[8]) {
   uint32_t h[4], l[4];
 #pragma unroll
@@ -49,7 +51,7 @@ __device__ __forceinline__ void store_split(uint32_t at, uint32_t low, const flo
     l[i] = half2_bits(x[2 * i] - back.x, x[2 * i + 1] - back.y);
   }
   sts128(at, h[0], h[1], h[2], h[3]);
-  sts128(at + low, l[0], l[1], l[2], l[3]);
+  if (low) sts128(at + low, l[0], l[1], l[2], l[3]);
 }
 __device__ __forceinline__ void sts_float(uint32_t a, float v) {
   asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(a), "f"(v) : "memory");
@@ -79,7 +81,7 @@ __device__ __forceinline__ int run_of(long long x, long long share) {
 }
 
 template <bool JOIN, int D>
-__global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms) {
+__global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms, int rows_per) {
   using M = Map<D>;
   extern __shared__ __align__(1024) uint8_t dyn_smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -117,7 +119,7 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms) 
     asm volatile("griddepcontrol.wait;\n" ::: "memory");   // the states
   }
   // ---- the rows: kPieces lanes a row, several rows of a warp at a time ------------------------------
-  const int64_t rows = (int64_t)p.B * p.Q * p.Hq, row0 = (int64_t)blockIdx.x * kRows;
+  const int64_t row0 = (int64_t)blockIdx.x * rows_per, rows = min((int64_t)p.B * p.Q * p.Hq, row0 + rows_per);
   constexpr int kPerWarp = 32 / kPieces, kStep = kThreads / 32 * kPerWarp;
   const int piece = lane % kPieces, first = warp * kPerWarp + lane / kPieces;
   // all of a thread's loads of queries go out before the first is used
@@ -141,6 +143,7 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms) 
 #pragma unroll
   for (int k = 0; k < kRows / kStep; ++k) {
     const int r = first + k * kStep;
+    if (k > 0 && k * kStep >= rows_per) break;              // (the same for all)
     const int64_t row = row0 + r;
     float x[8];
 #pragma unroll
@@ -214,7 +217,8 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms) 
     const float power = power_of(most, inverse);
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] *= inverse;
-    store_split(M::kA + (uint32_t)(r >> 3) * M::kGroup + (uint32_t)piece * 128u + (uint32_t)(r & 7) * 16u, M::kABytes, x);
+    store_split(M::kA + (uint32_t)(r >> 3) * M::kGroup + (uint32_t)piece * 128u + (uint32_t)(r & 7) * 16u,
+                terms > 2 ? M::kALow - M::kA : 0u, x);
     if (piece == 0) sts_float(M::kScales + 4u * r, power);
   }
   asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
@@ -227,7 +231,7 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms) 
     if (elect_one()) {
       constexpr uint32_t kIdesc = M::kIdesc | (JOIN ? 1u << 16 : 0u);       // states: Pi is MN-major
       for (int t = 0; t < terms; ++t) {                    // high x high, high x low, low x high
-        const uint64_t a = descriptor(M::kA + (t == 2 ? M::kABytes : 0u), 128u, M::kGroup);
+        const uint64_t a = descriptor(t == 2 ? M::kALow : M::kA, 128u, M::kGroup);
         const uint32_t from = M::kB + (t == 1 ? M::kBBytes : 0u);
         const uint64_t b = JOIN ? descriptor(from, M::kGroup, 128u) : descriptor(from, 128u, M::kGroup);
 #pragma unroll
@@ -304,9 +308,15 @@ template <bool JOIN, int D> int launch(const Params &p, cudaStream_t stream) {
     opted_in[dev & 63].store(true, std::memory_order_release);
   }
   const int64_t all = (int64_t)p.B * p.Q * p.Hq;
-  const int blocks = (int)((all + kRows - 1) / kRows), terms = JOIN || p.dtype == WTQ_F32 ? 3 : 2;
-  if (JOIN) return launch_behind(product_kernel<JOIN, D>, blocks, kThreads, M::kBytes, stream, "wtq_tree join launch", p, terms);
-  product_kernel<JOIN, D><<<blocks, kThreads, M::kBytes, stream>>>(p, terms);
+  // Few rows are spread over more blocks, as far as there are multiprocessors: a block's time is the
+  // chain of reads that its rows' pieces make (2688 rows of 8 pieces: 26 us on 21 blocks).
+  int rows_per = kRows;
+  while (rows_per > 16 && (all + rows_per / 2 - 1) / (rows_per / 2) <= device_sms()) rows_per /= 2;
+  const int blocks = (int)((all + rows_per - 1) / rows_per), terms = p.dtype == WTQ_F32 || (JOIN && p.dtype == WTQ_F16) ? 3 : 2;
+  const size_t bytes = terms > 2 ? M::kBytes : M::kALow;    // (two blocks a multiprocessor without low parts)
+  if (JOIN)
+    return launch_behind(product_kernel<JOIN, D>, blocks, kThreads, bytes, stream, "wtq_tree join launch", p, terms, rows_per);
+  product_kernel<JOIN, D><<<blocks, kThreads, bytes, stream>>>(p, terms, rows_per);
   note_launches(1);
   return check_cuda(cudaGetLastError(), "wtq_tree rotate launch");
 }
