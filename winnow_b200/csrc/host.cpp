@@ -392,8 +392,8 @@ PyObject *rope(PyObject *, PyObject *const *a, Py_ssize_t n) {
       positions.scalar_type() != at::kInt || positions.device() != dev || table.dim() != 2 || table.stride(1) != 1 ||
       table.scalar_type() != at::kFloat || table.device() != dev || table.size(1) > D || table.size(1) % 2)
     Py_RETURN_NONE;
-  const c10::cuda::OptionalCUDAGuard guard(dev);
-  if (a[9] != Py_None) {                  // given outputs: buffers of their own, else the Python path looks closer
+  const bool given = a[9] != Py_None;
+  if (given) {                            // buffers of their own, else the Python path looks closer
     if (!PyTuple_Check(a[9]) || PyTuple_GET_SIZE(a[9]) != sides) Py_RETURN_NONE;
     for (int i = 0; i < sides; ++i) {
       if (!tensor(PyTuple_GET_ITEM(a[9], i), y[i]) || y[i].sizes() != x[i].sizes() || y[i].stride(3) != 1 ||
@@ -403,9 +403,9 @@ PyObject *rope(PyObject *, PyObject *const *a, Py_ssize_t n) {
         if (y[i].storage().data() == x[j].storage().data() || (j < i && y[i].storage().data() == y[j].storage().data()))
           Py_RETURN_NONE;
     }
-  } else {
-    for (int i = 0; i < sides; ++i) y[i] = at::empty(x[i].sizes(), q.options());
   }
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  for (int i = 0; i < sides && !given; ++i) y[i] = at::empty(x[i].sizes(), q.options());
   wtq_rope_side_t s[3] = {};
   for (int i = 0; i < sides; ++i) {
     s[i].x = x[i].const_data_ptr();
@@ -465,8 +465,8 @@ PyObject *plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
   } else if (!fresh.defined() || !words(fresh, dev, {B})) {
     Py_RETURN_NONE;
   }
-  const c10::cuda::OptionalCUDAGuard guard(dev);
-  if (a[9] != Py_None) {
+  const bool given = a[9] != Py_None;
+  if (given) {
     if (!PyTuple_Check(a[9]) || PyTuple_GET_SIZE(a[9]) != 9 || !ticket.defined()) Py_RETURN_NONE;
     for (int i = 0; i < 9; ++i)
       if (!optional(PyTuple_GET_ITEM(a[9], i), o[i]) || (i < 8 && !o[i].defined())) Py_RETURN_NONE;
@@ -474,7 +474,9 @@ PyObject *plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
         !words(o[4], dev, {tokens}) || !words(o[5], dev, {tokens}) || !words(o[6], dev, {tokens, 1}) ||
         !words(o[7], dev, {tokens}) || (parents.defined() && (!o[8].defined() || !words(o[8], dev, {B, Q, words_of}))))
       Py_RETURN_NONE;
-  } else {
+  }
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  if (!given) {
     const at::Tensor buffer = at::empty({9 * 64 + 3 * B + 2 + 4 * tokens + B * Q * words_of}, lengths.options());
     int64_t at = 0;
     o[0] = cut(buffer, at, {B});

@@ -9,9 +9,29 @@ Inference only, like the rest of the package: there is no backward pass.
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
 
 from . import _lib
+
+
+@dataclass
+class Rotary:
+    """A model's position rotation, with the norms of its layers' queries and keys where it has them:
+    `q_weights[i]`, `k_weights[i]` (D,) of layer i, or None for no norm."""
+
+    table: torch.Tensor
+    q_weights: list | None = None
+    k_weights: list | None = None
+    eps: float = 1e-6
+    interleaved: bool = False
+
+    def apply(self, layer: int, q, k, positions, *, v=None, out=None, status=None):
+        """`qk_norm_rope` with what layer `layer` has."""
+        return qk_norm_rope(q, k, positions, self.table, eps=self.eps, interleaved=self.interleaved, v=v, out=out,
+                            q_weight=None if self.q_weights is None else self.q_weights[layer],
+                            k_weight=None if self.k_weights is None else self.k_weights[layer], status=status)
 
 
 def rotary_table(rot: int, positions: int, *, base: float = 10000.0, inv_freq: torch.Tensor | None = None,
