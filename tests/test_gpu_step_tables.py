@@ -198,6 +198,16 @@ def test_in_place_over_many_blocks():
         lens, held, count = want["seq_lens"], want["held"], want["free_count"][0]
 
 
+def test_rooms_of_ragged_steps():
+    """Any number of tokens, and no more tensors kept than there are powers of two."""
+    d = DevicePages(pool_of(200), "batch", pages=200, batch=2, width=100)
+    for n in [*range(0, 40), 100, 64, 65]:
+        p = d.extend(i32([n - n // 3, n // 3]), tokens=n)
+        assert p.slot_pages.shape == (n, 1) and p.sequence.tolist() == [0] * (n - n // 3) + [1] * (n // 3)
+    assert len(d._room) <= 8
+    d.check()
+
+
 def test_captured_steps():
     pool = pool_of(200)
     d = DevicePages(pool, "batch", pages=200, batch=3, width=60)

@@ -140,6 +140,29 @@ def test_nan_queries_of_padding_reach_nobody(dtype):
     assert torch.equal(clean, dirty)
 
 
+@pytest.mark.parametrize("lens", [[200, 90], [9000, 90]])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_query_that_is_not_a_number_spoils_its_own_row(dtype, lens):
+    kv = build(lens, 2, 128, 16, 4, 4)
+    mask = plain.words(trees(2, 6, 3)).to(DEV)
+    q = torch.randn(2, 8, 6, 128, generator=torch.Generator().manual_seed(5)).to(DEV, dtype)
+    clean = tree_decode_attention(q, kv, mask, 0.09)
+    q[0, 3, 2, 7] = float("nan")
+    q[1, 0, 0] = float("nan")
+    dirty = tree_decode_attention(q, kv, mask, 0.09)
+    assert dirty[0, 3, 2].isnan().all() and dirty[1, 0, 0].isnan().all()
+    dirty[0, 3, 2], dirty[1, 0, 0] = clean[0, 3, 2], clean[1, 0, 0]
+    assert torch.equal(clean, dirty)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_queries_beyond_fp16(dtype):
+    """|q| of 1e6: logits of 1e5 and more, all weight on one token, whose value comes back as it is stored
+    (fp16 centroid times norm: 2^-11 each at most)."""
+    kv = build([300, 40], 2, 128, 16, 4, 4)
+    check(kv, 2, 8, 5, dtype, mult=1e6, rel=1e-3 + (4e-3 if dtype == torch.bfloat16 else 0))
+
+
 def test_bits_past_the_tree_are_ignored():
     kv = build([200], 2, 128, 16, 4, 4)
     seen = trees(1, 5, 3)

@@ -140,8 +140,8 @@ class DevicePages:
 
     def extend(self, new_tokens=None, *, tokens: int | None = None, parents=None) -> TokenPlan:
         """Append new_tokens[b] tokens (`tokens` in all, or room for more), or a tree each.  The plan's
-        per-token tensors are this object's own, one set for each number of tokens, and written
-        again by the next call with that number; its state tensors are `lengths`, `held`, `free_count`."""
+        per-token tensors are this object's own and written again by a later call for about as many
+        tokens; its state tensors are `lengths`, `held`, `free_count`."""
         B = self.lengths.numel()
         if parents is not None:
             Q = int(parents.shape[1]) if parents.dim() == 2 else 0
@@ -150,12 +150,17 @@ class DevicePages:
             raise ValueError("extend needs the number of tokens: reading it off the device would wait")
         else:
             Q = 0
-        room = self._room.get((tokens, Q))
+        # (a captured step keeps its addresses: rooms are never given up, so there is one a power of two)
+        size = tokens if Q else 1 << max(tokens - 1, 0).bit_length()
+        room = self._room.get((size, Q))
         if room is None:
             e = lambda *shape: torch.empty(shape, dtype=torch.int32, device=self.pool.device)   # noqa: E731
-            room = self._room[(tokens, Q)] = TokenPlan(
-                self.lengths, self.held, self.free_count, e(B + 1), e(tokens), e(tokens), e(tokens, 1), e(tokens),
+            room = self._room[(size, Q)] = TokenPlan(
+                self.lengths, self.held, self.free_count, e(B + 1), e(size), e(size), e(size, 1), e(size),
                 e(B, Q, -(-Q // 32)) if Q else None)
+        if size != tokens:
+            room = room._replace(**{name: getattr(room, name)[:tokens]
+                                    for name in ("sequence", "positions", "slot_pages", "slot_ends")})
         return plan_tokens(self.lengths, new_tokens, self.table, self.held, self.free_pages, self.free_count,
                            self.page_size, tokens, parents=parents, out=room, ticket=self._ticket, status=self.status)
 

@@ -90,8 +90,8 @@ __global__ void __launch_bounds__(kRowThreads) join_kernel(Params p) {
     };
     if (c0 == c1) {
       const float l = p.l[row];
-      const float f = l > 0.f ? 1.f / l : 0.f;
-      for (int d = lane; d < p.D; d += 32) to[d] = l > 0.f ? p.acc[row * p.D + d] * f : 0.f;
+      const float f = l != 0.f ? 1.f / l : 0.f;
+      for (int d = lane; d < p.D; d += 32) to[d] = l != 0.f ? p.acc[row * p.D + d] * f : 0.f;
       continue;
     }
     float top = -INFINITY;
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kRowThreads) join_kernel(Params p) {
       if (p.part_m[s] != -INFINITY) sum += p.part_l[s] * exp2f(p.part_m[s] - top);
     }
     sum = warp_sum(sum);
-    const float f = sum > 0.f ? 1.f / sum : 0.f;
+    const float f = sum != 0.f ? 1.f / sum : 0.f;
     float x[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = 0.f;
@@ -299,6 +299,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(Params p) {
           const uint32_t seen = visible(words, p.Q, tok0 - hist);
           const float v = (seen >> lane & 1u) != 0 && tok0 + lane < L ? ps[r * kP + lane] : -INFINITY;
           const float now = fmaxf(m[k], warp_max(v));
+          if (now == -INFINITY && __any_sync(0xffffffffu, v != v)) l[k] = NAN;
           if (now != -INFINITY) {
             f = m[k] == -INFINITY ? 0.f : exp2f(m[k] - now);
             w = v == -INFINITY ? 0.f : exp2f(v - now);
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(Params p) {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       if (lane == 0 && place(8 * warp + k, at, at_m, at_l)) {
-        *at_m = m[k];
+        *at_m = l[k] != l[k] ? 0.f : m[k];                // a query that is not a number: so is its result
         *at_l = l[k];
       }
 #pragma unroll

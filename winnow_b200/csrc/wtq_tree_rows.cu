@@ -90,7 +90,6 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms, 
     if (p.status && tid == 0) atomicOr(p.status, WTQ_STATUS_LAYOUT);
     return;
   }
-  if (!JOIN) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   constexpr int kPieces = D / 8;
   const float *Pi = JOIN ? p.v.Pi : p.k.Pi;
   if (warp == 0) {
@@ -101,6 +100,12 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms, 
   if (tid == 0) {
     mbar_init(M::kBar, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if constexpr (!JOIN) {
+    // Only now that this block has its tensor memory: a block of the scan that took all of it first would
+    // wait for this kernel while this block waited for it.
+    __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   }
 #pragma unroll
   for (int e = tid; e < D * kPieces; e += kThreads) {
@@ -176,14 +181,14 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms, 
       const long long g0 = (long long)prefix[b] * p.row_blocks * p.Hkv + (long long)(rb * p.Hkv + kvh) * n;
       const int c0 = n > 0 ? run_of(g0, share) : 0, c1 = n > 0 ? run_of(g0 + n - 1, share) : -1;
       auto add = [&](const float *acc, float w) {
-        const float4 a = __ldg(reinterpret_cast<const float4 *>(acc + 8 * piece));
-        const float4 c = __ldg(reinterpret_cast<const float4 *>(acc + 8 * piece) + 1);
+        const float4 a = __ldcg(reinterpret_cast<const float4 *>(acc + 8 * piece));
+        const float4 c = __ldcg(reinterpret_cast<const float4 *>(acc + 8 * piece) + 1);
         x[0] = fmaf(w, a.x, x[0]); x[1] = fmaf(w, a.y, x[1]); x[2] = fmaf(w, a.z, x[2]); x[3] = fmaf(w, a.w, x[3]);
         x[4] = fmaf(w, c.x, x[4]); x[5] = fmaf(w, c.y, x[5]); x[6] = fmaf(w, c.z, x[6]); x[7] = fmaf(w, c.w, x[7]);
       };
       if (c0 == c1) {                                       // an empty state's accumulator is not read
         const float l = p.l[row];
-        if (l > 0.f) add(p.acc + row * D, 1.f / l);
+        if (l != 0.f) add(p.acc + row * D, 1.f / l);
       } else if (c0 < c1) {
         // the row's lanes look at a piece each; then all add up its coordinates, piece by piece
         auto state = [&](int c) -> int64_t { return ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * p.rows + qr - rb * p.rows; };
@@ -196,7 +201,7 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms, 
           const int c = from + piece;
           const float m = c <= c1 ? p.part_m[state(c)] : -INFINITY;
           const float w = m == -INFINITY ? 0.f : exp2f(m - top);
-          if (w > 0.f) sum = fmaf(w, p.part_l[state(c)], sum);
+          if (w != 0.f) sum = fmaf(w, p.part_l[state(c)], sum);
           const int last = min(kPieces, c1 - from + 1);
 #pragma unroll 8
           for (int e = 0; e < last; ++e)                    // (a live row's accumulators are all written)
@@ -204,9 +209,9 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms, 
         }
 #pragma unroll
         for (int o = kPieces / 2; o; o >>= 1) sum += __shfl_xor_sync(group, sum, o);
-        const float f = sum > 0.f ? 1.f / sum : 0.f;
+        const float f = sum != 0.f ? 1.f / sum : 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = sum > 0.f ? x[e] * f : 0.f;
+        for (int e = 0; e < 8; ++e) x[e] = sum != 0.f ? x[e] * f : 0.f;
       }
     }
     float most = 0.f, inverse;

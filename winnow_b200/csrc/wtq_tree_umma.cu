@@ -23,8 +23,8 @@
 // A warp on its own gets through an instruction in about nine cycles here, so a role is only as fast
 // as its instructions per tile are few.
 //
-// fp16 scores carry an error that grows with |q| |k|; a warp whose tile holds a row maximum beyond
-// kPreciseAbove (log2 domain) recomputes that tile's scores in fp32 from the packed codes.
+// fp16 scores carry an error that grows with |q| |k|; rows whose maximum in a tile lies beyond
+// kPreciseAbove (log2 domain) take that tile's scores in fp32 from the packed codes.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -256,12 +256,14 @@ __device__ __noinline__ uint2 seen_tokens(const Params &p, int b, int qr, int at
 }
 
 // fp32 scores of query row `qr` (negative: zeros) with the 64 tokens from `tok0` on, from the packed codes,
-// the same addresses for the whole warp, to `own`; those it does not see are -inf.
+// the same addresses for the whole warp, to `own` where they are wanted; those it does not see are -inf.
 // Out of line: only for tiles whose scores came out large.
 template <int BW, int D>
-__device__ __noinline__ void precise_scores(const Params &p, Piece c, int qr, int tok0, uint2 seen, float *own) {
+__device__ __noinline__ void precise_scores(const Params &p, Piece c, int qr, int tok0, bool masked, bool wanted, float *own) {
   constexpr int kRowBytes = D * BW / 8;
   const int end = length_of(p, c.b), i = qr / p.n_rep;
+  uint2 seen = make_uint2(kFull, kFull);
+  if (masked && qr >= 0) seen = seen_tokens(p, c.b, qr, tok0 - (end - p.Q));
   const float *q = qr < 0 ? nullptr : p.q_rot + (((int64_t)c.b * p.Q + i) * p.Hq + c.h * p.n_rep + qr - i * p.n_rep) * D;
 #pragma unroll 1
   for (int blk = 0; blk < kTile / 16; ++blk) {                 // sixteen tokens of one page
@@ -275,7 +277,7 @@ __device__ __noinline__ void precise_scores(const Params &p, Piece c, int qr, in
                            (int64_t)(tok % p.S) * kRowBytes;
 #pragma unroll 1
       for (int d = 0; d < D / 4; ++d) {                        // four coordinates: BW / 2 bytes of each row
-        const float4 x = q ? __ldg(reinterpret_cast<const float4 *>(q) + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 x = q ? __ldcg(reinterpret_cast<const float4 *>(q) + d) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           uint32_t w = 0;
@@ -294,7 +296,8 @@ __device__ __noinline__ void precise_scores(const Params &p, Piece c, int qr, in
     }
     const uint32_t bits = (blk < 2 ? seen.x : seen.y) >> (16 * (blk & 1));
 #pragma unroll
-    for (int k = 0; k < 16; ++k) own[16 * blk + k] = (bits >> k & 1u) ? acc[k] : -INFINITY;
+    for (int k = 0; k < 16; ++k)
+      if (wanted) own[16 * blk + k] = (bits >> k & 1u) ? acc[k] : -INFINITY;
   }
 }
 
@@ -324,7 +327,6 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D>::kThreads, 1) scan_kernel(con
     if (p.status && tid == 0) atomicOr(p.status, WTQ_STATUS_LAYOUT);
     return;
   }
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   int *prefix = reinterpret_cast<int *>(dyn_smem + (kPrefix - (uint32_t)__cvta_generic_to_shared(dyn_smem)));
   for (int e = tid; e < M::kEntries * 64; e += M::kThreads)
     sts32(mma::kLutAddr + 4u * e, mma::lut_word(e, BWK, BWV, p.k.centroids, p.v.centroids));
@@ -359,6 +361,9 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D>::kThreads, 1) scan_kernel(con
   fence_before();
   tile_prefix(p, prefix);                                   // (ends with a block barrier)
   fence_after();
+  // Only now: the join's blocks take tensor memory too, and one that got it before this block's share was
+  // taken would wait for this kernel's end while this block waited for it.
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   const uint32_t tmem = lds32(kTmemSlot);
   const long long share = run_length(p, prefix), all = (long long)prefix[p.B] * p.row_blocks * p.Hkv;
   const long long begin = share * blockIdx.x, end = min(all, begin + share);
@@ -397,7 +402,7 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D>::kThreads, 1) scan_kernel(con
         uint32_t v[kPart / 2];
 #pragma unroll
         for (int k = 0; k < kPart / 4; ++k) {
-          const float4 y = q ? __ldg(reinterpret_cast<const float4 *>(q + kPart * st) + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float4 y = q ? __ldcg(reinterpret_cast<const float4 *>(q + kPart * st) + k) : make_float4(0.f, 0.f, 0.f, 0.f);
           v[2 * k] = pack_half2(y.x, y.y);
           v[2 * k + 1] = pack_half2(y.z, y.w);
         }
@@ -429,18 +434,23 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D>::kThreads, 1) scan_kernel(con
         __syncwarp();
         if (lane == 0) mbar_arrive(kSFree + 8u * st);       // the scores are in registers
         const bool masked = tok0 + kTile > hist;
-        uint2 seen = make_uint2(kFull, kFull);
+        bool sees = live;
         if (masked) {
+          uint2 seen = make_uint2(kFull, kFull);
           if (live) seen = seen_tokens(p, c.b, qr, tok0 - hist);
           hide(s, seen);
+          sees = live && (seen.x | seen.y) != 0u;
         }
         float mx = maximum(s);
-        const bool large = !(fabsf(mx) <= kPreciseAbove) && mx != -INFINITY;
+        // (no maximum although something is seen: scores that are not numbers, as of a query beyond fp16)
+        const bool large = !(fabsf(mx) <= kPreciseAbove) && (mx != -INFINITY || sees);
         bool drained = k == 0;                              // the stream's last products have ended
         if (__any_sync(kFull, large || mx > ref + kSlack || (ref == -INFINITY && mx != -INFINITY))) {
           if (__any_sync(kFull, large)) {
             float own[64];
-            precise_scores<BWK, D>(p, c, live ? qr : -1, tok0, seen, own);
+#pragma unroll
+            for (int e = 0; e < 64; ++e) own[e] = __uint_as_float(s[e]);
+            precise_scores<BWK, D>(p, c, live ? qr : -1, tok0, masked, large, own);
 #pragma unroll
             for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(own[e]);
             mx = maximum(s);
@@ -497,9 +507,13 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D>::kThreads, 1) scan_kernel(con
       ok = __all_sync(kFull, ok && lds32(kAbort) == 0u);
       if (ok) {
         auto state = [&](int what) { return __uint_as_float(lds32(kStates + 4u * (what * kRows + r))); };
-        const float m0 = state(0), m1 = state(2), top = fmaxf(m0, m1);
+        const float m0 = state(0), m1 = state(2);
+        float top = fmaxf(m0, m1);
+        const float l0 = state(1), l1 = state(3);
+        const bool broken = l0 != l0 || l1 != l1;           // a query that is not a number: so is its result
         const float w0 = m0 == -INFINITY ? 0.f : ex2(m0 - top), w1 = m1 == -INFINITY ? 0.f : ex2(m1 - top);
-        const float total = w0 * state(1) + w1 * state(3);
+        const float total = broken ? l0 + l1 : w0 * l0 + w1 * l1;
+        if (broken) top = 0.f;
         float *acc;
         const int64_t row = row_of();
         if (c.slot < 0) {
