@@ -345,7 +345,8 @@ int wtq_release_tokens(const int32_t *marks, int32_t *table, int64_t table_strid
  * history, and tree tokens before its position 0 do not exist.  fp32 queries are computed in fp32 on the
  * CUDA cores; 16-bit queries on the tensor cores (fp16 operands, fp32 sums) where head_dim is 64 or 128,
  * the widths 4/4, 4/6, 6/6 or 8/8, the page size a power of two >= 16 and the pages 16-byte aligned,
- * otherwise in fp32 as well.  head_dim <= 256, B <= 2048 x 65535.  Status bits as for wtq_decode.  The
+ * otherwise in fp32 as well.  head_dim <= 256, B Q <= 2^24, B Q Hq < 2^31, max_pages S <= 2^30.  A tree
+ * token whose norms are not finite reaches the tokens that see it only.  Status bits as for wtq_decode.  The
  * workspace (wtq_tree_workspace_bytes, 256-byte aligned) needs no preparation. */
 size_t wtq_tree_workspace_bytes(int B, int Hq, int Hkv, int Q, int D);
 int wtq_tree(const void *q, int dtype, const int64_t q_strides[3], void *out, const int64_t out_strides[3],
@@ -360,7 +361,9 @@ int wtq_tree_on_tensor_cores(const wtq_side_t *k_side, const wtq_side_t *v_side,
  * token i for i < counts[b] (keep ascends; (B, most), row stride in elements), in every layer, as the
  * codes and norms it has; out[b] = seq_lens[b] - drafted + counts[b].  out must not be seq_lens.  A path
  * that does not ascend or leaves the tree keeps nothing of it (out[b] = seq_lens[b] - drafted; where that
- * is negative, seq_lens[b]) and sets WTQ_STATUS_BAD_POSITION. */
+ * is negative, seq_lens[b]) and sets WTQ_STATUS_BAD_POSITION.  `granted` may be null; else it is a word
+ * that is 0 if the trees were refused (starts[B] of their plan): nothing is kept or cut off then, out =
+ * seq_lens. */
 typedef struct {
   uint8_t *pages;            /* all layers: (layers, P, Hkv, S, row_bytes) */
   void *norms;               /* fp16 (layers, P, Hkv, S) */
@@ -371,7 +374,7 @@ typedef struct {
 int wtq_keep_tokens(const wtq_pool_side_t *k_side, const wtq_pool_side_t *v_side, const int32_t *page_table,
                     int64_t table_stride, const int32_t *seq_lens, const int32_t *keep, int64_t keep_stride,
                     const int32_t *counts, int layers, int B, int Hkv, int S, int P, int max_pages, int most,
-                    int drafted, int32_t *out, int32_t *status, void *stream);
+                    int drafted, const int32_t *granted, int32_t *out, int32_t *status, void *stream);
 
 /* Replaces tq_dequant / tq_dequant_cuda (turboquant_kv/kernel.py:78-115,
  * turboquant_kv/csrc/tq_dequant.cu:186-211): N packed rows -> (N, D) of

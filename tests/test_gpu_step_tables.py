@@ -86,10 +86,10 @@ def refused(p, lens, held, count, status, bit):
     assert not p.slot_ends.any()
 
 
-@pytest.mark.parametrize("why", ["pages", "width", "tokens", "negative", "held", "count"])
+@pytest.mark.parametrize("why", ["pages", "width", "tokens", "negative", "held", "count", "far"])
 def test_refused_steps_take_nothing(why):
     lens, held, new, count, tokens, W = [20, 5], [2, 1], [30, 3], 4, 40, 8
-    bit = _lib.STATUS_BAD_POSITION
+    S, bit = 16, _lib.STATUS_BAD_POSITION
     if why == "pages":
         count, bit = 1, _lib.STATUS_NO_PAGES
     elif why == "width":
@@ -100,11 +100,13 @@ def test_refused_steps_take_nothing(why):
         lens = [20, -1]
     elif why == "held":
         held = [2, 9]
+    elif why == "far":
+        lens, S, W = [2 ** 31 - 20, 5], 2 ** 28, 8
     else:
         count = 5
     free = [9, 8, 7, 6]
     t, status = torch.full((2, W), -1, dtype=torch.int32, device=DEV), i32([0])
-    p = plan_tokens(i32(lens), i32(new), t, i32(held), i32(free), i32([count]), 16, tokens, status=status)
+    p = plan_tokens(i32(lens), i32(new), t, i32(held), i32(free), i32([count]), S, tokens, status=status)
     refused(p, lens, held, count, status, bit)
     assert (t == -1).all()
 
@@ -299,3 +301,14 @@ def test_keep_strided_pools():
     assert keep_tokens(*pool, i32([[4, 0]]), i32([30]), i32([[1, 4, 9]]), i32([3]), 14).tolist() == lengths
     assert all(torch.equal(a, b) for a, b in zip(pool, want))
     assert torch.equal(wide[:, :, 2], before[:, :, 2]) and torch.equal(wide[..., :4], before[..., :4])
+
+
+def test_refused_trees_keep_their_history():
+    pool = random_pool(4, 1, 2, 16, 64, 64, seed=2)
+    before = [t.clone() for t in pool]
+    for granted, want in ((0, [20]), (8, [14])):
+        got = keep_tokens(*pool, i32([[0, 1]]), i32([20]), i32([[0, 5]]), i32([2]), 8, granted=i32([granted]))
+        assert got.tolist() == want
+        assert all(torch.equal(a, b) for a, b in zip(pool, before)) == (granted == 0)
+    with pytest.raises(ValueError):
+        keep_tokens(*pool, i32([[0, 1]]), i32([20]), i32([[0, 5]]), i32([2]), 8, granted=i32([1, 1]))

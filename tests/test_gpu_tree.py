@@ -278,3 +278,44 @@ def test_more_sequences_than_a_launch_takes():
     B = 2050
     kv = build([20] * B, 1, 64, 16, 4, 4)
     check(kv, B, 2, 2, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype,widths", [(torch.float32, (4, 4)), (torch.bfloat16, (4, 4)), (torch.bfloat16, (8, 8)),
+                                          (torch.bfloat16, (4, 6))])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_norms_that_are_not_numbers_reach_those_that_see_them(dtype, widths, bad):
+    """Tree tokens with such norms: siblings and tokens after them keep their bits, descendants are NaN."""
+    lens, Q = [200, 73, 3000], 13
+    kv = build(lens, 2, 128, 16, *widths)
+    seen = trees(3, Q, 5)
+    q = torch.randn(3, 8, Q, 128, generator=torch.Generator().manual_seed(3)).to(DEV, dtype)
+    mask = plain.words(seen).to(DEV)
+    want = tree_decode_attention(q, kv, mask, 0.09)
+    spoilt = torch.zeros(3, Q, dtype=torch.bool)
+    for b, L in enumerate(lens):
+        for j in (4, 9):
+            at = L - Q + j
+            page = int(kv.page_table[b, at // 16])
+            kv.v_norms[page, :, at % 16] = bad
+            if j == 9:
+                kv.k_norms[page, :, at % 16] = bad
+            spoilt[b] |= seen[b, :, j]
+    assert spoilt.any() and not spoilt.all()
+    got = tree_decode_attention(q, kv, mask, 0.09).transpose(1, 2)
+    spoilt = spoilt.to(DEV)
+    assert got[spoilt].isnan().all()
+    assert torch.equal(got[~spoilt], want.transpose(1, 2)[~spoilt])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("at", [5, 4000, 8900])
+def test_a_norm_in_the_history_that_is_not_a_number_is_not_lost(dtype, at):
+    """One in a long history, whose other pieces may have far larger maxima: every row sees it."""
+    kv = build([9000, 90], 2, 128, 16, 4, 4)
+    q = (100 * torch.randn(2, 8, 3, 128, generator=torch.Generator().manual_seed(3))).to(DEV, dtype)
+    mask = plain.words(trees(2, 3, 1)).to(DEV)
+    want = tree_decode_attention(q, kv, mask, 0.09)
+    kv.v_norms[int(kv.page_table[0, at // 16]), 1, at % 16] = float("inf")
+    got = tree_decode_attention(q, kv, mask, 0.09)
+    assert got[0, 4:].isnan().all()
+    assert torch.equal(got[0, :4], want[0, :4]) and torch.equal(got[1], want[1])

@@ -211,3 +211,51 @@ def test_a_position_past_the_table_is_reported():
     s.layer(0, k, v, q)
     with pytest.raises(StalePage):
         s.check()
+
+
+def test_a_refused_step_leaves_the_histories():
+    """More pages than are free: nothing is appended, kept or cut off, and the step says so."""
+    pool, d, s, rotary, kq, vq = build(torch.bfloat16, pages=6)
+    prompt(d, kq, vq, rotary, [[1] * 30, [2] * 31, [3] * 29], torch.bfloat16)
+    def state():
+        return [t.clone() for t in (d.lengths, d.held, d.free_count, d.table, *pool.layer(0), *pool.layer(1))]
+    before = state()
+    p = s.begin(i32([[-1, 0, 1, 2, 3, 4, 5, 6, 7]] * B))
+    q, k, v = projections([[1] * 9] * B, 0, torch.bfloat16)
+    for layer in range(LAYERS):
+        assert not s.layer(layer, k, v, q).any()
+    assert s.accept(i32([[0, 1]] * B), i32([2, 1, 0])).tolist() == [30, 31, 29]
+    assert all(torch.equal(a, b) for a, b in zip(state(), before)) and not p.mask.any()
+    with pytest.raises(PoolExhausted):
+        s.check()
+    with pytest.raises(RuntimeError):
+        s.accept(i32([[0, 1]] * B), i32([2, 1, 0]))
+
+
+def test_a_step_without_a_rotary_takes_any_strides():
+    _, d, s, _, kq, vq = build(torch.float32)
+    s.rotary = None
+    parents = i32([[-1, 0, 1, 1, 3, 0, 5, 6, -2]] * B)
+    outs = []
+    q, k, v = projections([[i + 10 * b for i in range(9)] for b in range(B)], 0, torch.float32)
+    for make in (lambda t: t, lambda t: t.contiguous()):
+        s.begin(parents)
+        outs.append(s.layer(0, make(k), make(v), make(q)).clone())
+        s.accept(i32([[0]] * B), i32([0] * B))
+    s.check()
+    assert torch.equal(*outs) and outs[0].any()
+
+
+def test_padding_that_is_not_a_number_reaches_nobody():
+    """The projections of padding hold whatever they hold."""
+    pool, d, s, rotary, kq, vq = build(torch.bfloat16)
+    parents = i32([[-1, 0, 1, 1, 3, 0, 5, -2, -2], [-2] * 9, [-1, 0, -2, 0, -2, -2, 0, 6, -2]])
+    outs = []
+    for bad in (0.0, float("nan"), float("inf")):
+        p = s.begin(parents)
+        q, k, v = projections([[i + 10 * b for i in range(9)] for b in range(B)], 0, torch.bfloat16)
+        for t in (q, k, v):
+            t.transpose(1, 2)[parents == -2] = bad
+        outs.append(s.layer(0, k, v, q).clone())
+        s.accept(i32([[0]] * B), i32([0] * B))
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2]) and outs[0].isfinite().all()

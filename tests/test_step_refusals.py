@@ -106,7 +106,7 @@ def _keep(**kw):
     side = _lib.PoolSide(a["pages"], a["norms"], 64, 64, 64, 16, 16, 16, a["row"])
     return _lib.lib().wtq_keep_tokens(ctypes.byref(side), ctypes.byref(side), a["table"], 3, a["lens"], a["keep"], 2,
                                       a["counts"], a["layers"], a["B"], a["Hkv"], a["S"], a["P"], a["W"], a["most"],
-                                      a["drafted"], a["out"], None, None)
+                                      a["drafted"], None, a["out"], None, None)
 
 
 @pytest.mark.parametrize("bad", [dict(pages=None), dict(norms=None), dict(row=0), dict(table=None), dict(lens=None),

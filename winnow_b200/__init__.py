@@ -3,7 +3,8 @@
 
 Modules keep the reference's names: packing, cache, page_pool,
 packed_attention, packed_attention_cuda (in place of packed_attention_triton),
-packed_backend, dispatch.  Every operator needs CUDA tensors and the built
+packed_backend, dispatch.  Beside them: block_tables, rotary and engine_step (serving
+steps, speculative ones among them).  Every operator needs CUDA tensors and the built
 libwinnow_tq.so; nothing falls back to the CPU.
 """
 __version__ = "0.1.0"

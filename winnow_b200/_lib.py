@@ -135,7 +135,7 @@ _SIGNATURES = {
     "wtq_tree_on_tensor_cores": (c_int, [ctypes.POINTER(Side), ctypes.POINTER(Side), c_int, c_int, c_int]),
     "wtq_keep_tokens": (c_int, [ctypes.POINTER(PoolSide), ctypes.POINTER(PoolSide), c_void_p, c_int64, c_void_p,
                                 c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-                                c_void_p, c_void_p, c_void_p]),
+                                c_void_p, c_void_p, c_void_p, c_void_p]),
     "wtq_dequant": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                             c_int64, c_int64, c_int64, c_void_p]),
     "wtq_dequant_mode": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,

@@ -164,15 +164,16 @@ class DevicePages:
         return plan_tokens(self.lengths, new_tokens, self.table, self.held, self.free_pages, self.free_count,
                            self.page_size, tokens, parents=parents, out=room, ticket=self._ticket, status=self.status)
 
-    def keep(self, keep: torch.Tensor, counts: torch.Tensor, drafted: int) -> torch.Tensor:
+    def keep(self, keep: torch.Tensor, counts: torch.Tensor, drafted: int, plan: TokenPlan | None = None) -> torch.Tensor:
         """Of the last `drafted` tokens of every sequence, keep token keep[b][i] as its i-th for
-        i < counts[b], in every layer of the pool, and shorten `lengths` (`keep_tokens`)."""
+        i < counts[b], in every layer of the pool, and shorten `lengths` (`keep_tokens`).  With the step's
+        `plan`, a step that was refused leaves everything as it is."""
         from .packed_backend import keep_tokens
         pool = self.pool
         if pool.dense:
             raise ValueError("keep serves packed pools")
         after = keep_tokens(pool.k_pages, pool.k_norms, pool.v_pages, pool.v_norms, self.table, self.lengths, keep,
-                            counts, drafted, status=self.status)
+                            counts, drafted, granted=None if plan is None else plan.starts[-1:], status=self.status)
         self.lengths.copy_(after)
         return self.lengths
 

@@ -365,7 +365,7 @@ PyObject *rope(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   at::Tensor x[3], y[3], w[2], positions, table, status_tensor;
   if (n != 11 || !tensor(a[0], x[0]) || !tensor(a[1], x[1]) || !optional(a[2], x[2]) || !tensor(a[3], positions) ||
-      !tensor(a[4], table) || !optional(a[5], w[0]) || !optional(a[6], w[1]) || !PyFloat_Check(a[7]))
+      !tensor(a[4], table) || !optional(a[5], w[0]) || !optional(a[6], w[1]) || !PyFloat_Check(a[7]) || !PyBool_Check(a[8]))
     Py_RETURN_NONE;
   const int sides = x[2].defined() ? 3 : 2;
   const at::Tensor &q = x[0];
@@ -397,7 +397,7 @@ PyObject *rope(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (!PyTuple_Check(a[9]) || PyTuple_GET_SIZE(a[9]) != sides) Py_RETURN_NONE;
     for (int i = 0; i < sides; ++i) {
       if (!tensor(PyTuple_GET_ITEM(a[9], i), y[i]) || y[i].sizes() != x[i].sizes() || y[i].stride(3) != 1 ||
-          y[i].scalar_type() != q.scalar_type() || y[i].device() != dev || !y[i].is_contiguous())
+          y[i].scalar_type() != q.scalar_type() || y[i].device() != dev || !y[i].is_non_overlapping_and_dense())
         Py_RETURN_NONE;
       for (int j = 0; j < sides; ++j)
         if (y[i].storage().data() == x[j].storage().data() || (j < i && y[i].storage().data() == y[j].storage().data()))
@@ -419,7 +419,7 @@ PyObject *rope(PyObject *, PyObject *const *a, Py_ssize_t n) {
   }
   void *stream = (void *)at::cuda::getCurrentCUDAStream(dev.index()).stream();
   const float eps = (float)PyFloat_AS_DOUBLE(a[7]);
-  const int turned = PyObject_IsTrue(a[8]) > 0;
+  const int turned = a[8] == Py_True;
   int rc;
   {
     const Unlocked u;
@@ -560,13 +560,14 @@ PyObject *tree(PyObject *, PyObject *const *a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// keep(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, counts, drafted, out, status) -> lengths, or None
+// keep(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, counts, drafted, granted, out, status) -> lengths,
+// or None
 PyObject *keep(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  at::Tensor pages[2], norms[2], table, lens, path, counts, out, status_tensor;
-  if (n != 11 || !tensor(a[0], pages[0]) || !tensor(a[1], norms[0]) || !tensor(a[2], pages[1]) || !tensor(a[3], norms[1]) ||
+  at::Tensor pages[2], norms[2], table, lens, path, counts, granted, out, status_tensor;
+  if (n != 12 || !tensor(a[0], pages[0]) || !tensor(a[1], norms[0]) || !tensor(a[2], pages[1]) || !tensor(a[3], norms[1]) ||
       !tensor(a[4], table) || !tensor(a[5], lens) || !tensor(a[6], path) || !tensor(a[7], counts) || !PyLong_Check(a[8]) ||
-      !optional(a[9], out))
+      !optional(a[9], granted) || !optional(a[10], out))
     Py_RETURN_NONE;
   const int64_t drafted = PyLong_AsLongLong(a[8]);
   if (PyErr_Occurred()) {
@@ -577,7 +578,7 @@ PyObject *keep(PyObject *, PyObject *const *a, Py_ssize_t n) {
   int32_t *status;
   if (!pages[0].is_cuda() || drafted < 0 || drafted > INT32_MAX || table.dim() != 2 || table.scalar_type() != at::kInt ||
       table.stride(1) != 1 || table.device() != dev || table.size(0) < 1 || table.size(1) < 1 ||
-      !optional_status(a[10], dev, status_tensor, status))
+      (granted.defined() && !words(granted, dev, {1})) || !optional_status(a[11], dev, status_tensor, status))
     Py_RETURN_NONE;
   const int64_t B = table.size(0);
   wtq_pool_side_t s[2];
@@ -605,7 +606,8 @@ PyObject *keep(PyObject *, PyObject *const *a, Py_ssize_t n) {
                          path.const_data_ptr<int32_t>(), path.stride(0), counts.const_data_ptr<int32_t>(),
                          (int)pages[0].size(0), (int)B, (int)pages[0].size(2), (int)pages[0].size(3),
                          (int)pages[0].size(1), (int)table.size(1), (int)path.size(1), (int)drafted,
-                         out.mutable_data_ptr<int32_t>(), status, stream);
+                         granted.defined() ? granted.const_data_ptr<int32_t>() : nullptr, out.mutable_data_ptr<int32_t>(),
+                         status, stream);
   }
   if (rc) return library_error(rc);
   return THPVariable_Wrap(out);
@@ -630,7 +632,7 @@ PyMethodDef methods[] = {
      "plan(lengths, new_tokens, table, held, free_pages, free_count, page_size, tokens, parents, out, ticket, status)"},
     {"tree", (PyCFunction)(void (*)(void))tree, METH_FASTCALL, "tree(q, kv, mask, scale, out, workspace, status)"},
     {"keep", (PyCFunction)(void (*)(void))keep, METH_FASTCALL,
-     "keep(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, counts, drafted, out, status)"},
+     "keep(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, counts, drafted, granted, out, status)"},
     {"set_error", set_error, METH_O, "the exception type library errors are raised as"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "native host side of winnow_b200", -1, methods};

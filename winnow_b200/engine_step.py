@@ -34,7 +34,7 @@ from . import _lib
 from . import packed_attention as pa
 from .block_tables import DevicePages, TokenPlan
 from .packed_attention_cuda import DecodePlan, decode_workspace, tree_decode_attention, tree_workspace_bytes
-from .packed_backend import AppendPlan, append_tokens
+from .packed_backend import AppendPlan, append_planned
 from .page_pool import DeviceTable, PagePool, StalePage
 from .rotary import Rotary
 
@@ -160,7 +160,9 @@ class TreeSession:
     `pages`, `layer()` runs a layer's append and attention of all drafted tokens, `accept()` keeps a path
     of each tree.  Every part is launches on the current stream; the host waits for nothing, so a step
     can be captured in a CUDA graph.  Slots of the batch without a request are given all-padding trees
-    (parents -2): their tokens take places that `accept` with a count of 0 gives back."""
+    (parents -2): their tokens take places that `accept` with a count of 0 gives back.  A step that the
+    free pages do not cover runs through without an effect on the cache, its outputs are zeros, and
+    `check()` raises."""
 
     def __init__(self, pages: DevicePages, *, k_quant, v_quant, head_dim: int, q_heads: int, dtype: torch.dtype,
                  drafted: int, scale: float | None = None, rotary: Rotary | None = None):
@@ -173,8 +175,8 @@ class TreeSession:
             raise ValueError("drafted must be at least 1")
         self.pages, self.kq, self.vq, self.rotary, self.drafted = pages, k_quant, v_quant, rotary, Q
         self.scale = float(scale if scale is not None else D ** -0.5)
-        self.k_in = torch.zeros(B, Hkv, Q, D, dtype=dtype, device=dev)
-        self.v_in = torch.zeros(B, Hkv, Q, D, dtype=dtype, device=dev)
+        self.k_in = torch.zeros(B, Q, Hkv, D, dtype=dtype, device=dev).transpose(1, 2)
+        self.v_in = torch.zeros(B, Q, Hkv, D, dtype=dtype, device=dev).transpose(1, 2)
         self.q_in = torch.zeros(B, q_heads, Q, D, dtype=dtype, device=dev)
         self.out = torch.zeros(B, Q, q_heads, D, dtype=dtype, device=dev).transpose(1, 2)
         self.workspace = torch.empty(tree_workspace_bytes(B, q_heads, Hkv, Q, D, dev), dtype=torch.uint8, device=dev)
@@ -202,15 +204,18 @@ class TreeSession:
             positions = self.plan.positions.view(-1, self.drafted)
             q, k, v = self.rotary.apply(layer_idx, q, k, positions, v=v, out=(self.q_in, self.k_in, self.v_in),
                                         status=status)
-        append_tokens(k, v, kv.k_pages, kv.k_norms, kv.v_pages, kv.v_norms, kv.page_table, kv.seq_lens, self.kq,
-                      self.vq, status=status)
+        # (to the plan's slots, of which a refused step has none, so that it leaves the histories as they are)
+        k, v = (t.transpose(1, 2).reshape(-1, t.shape[1], t.shape[3]) for t in (k, v))
+        append_planned(k, v, kv.k_pages, kv.k_norms, kv.v_pages, kv.v_norms, self.plan, self.kq, self.vq, status=status)
         return tree_decode_attention(q, kv, self.plan.mask, self.scale, check_page_ids=False, out=self.out,
                                      workspace=self.workspace, status=status)
 
     def accept(self, keep: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
         """Keep tokens keep[b][:counts[b]] (ascending) of every tree; returns the new lengths."""
-        self.plan = None
-        return self.pages.keep(keep, counts, self.drafted)
+        if self.plan is None:
+            raise RuntimeError("begin() comes before accept()")
+        plan, self.plan = self.plan, None
+        return self.pages.keep(keep, counts, self.drafted, plan)
 
     def check(self) -> None:
         """Raise if a launch since the last check refused something (synchronises)."""

@@ -285,7 +285,7 @@ def append_planned(k, v, k_pages, k_norms, v_pages, v_norms, plan, k_tq, v_tq, *
 
 @torch.no_grad()
 def keep_tokens(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, counts, drafted: int, *,
-                out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+                granted: torch.Tensor | None = None, out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
     """Keep a path of every sequence's last `drafted` tokens: token keep[b][i] becomes token i of them
     for i < counts[b], in every layer, codes and norms as they are (`wtq_keep_tokens`); returns the
     lengths after it, seq_lens - drafted + counts.
@@ -293,9 +293,10 @@ def keep_tokens(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, 
     pages (layers, P, Hkv, S, NB) uint8, norms (layers, P, Hkv, S) fp16: a `PagePool`'s; page_table
     (B, W), seq_lens (B,), counts (B,) and keep (B, A) int32, each row of keep ascending (what follows
     its counts[b] entries is not read).  A row that does not ascend or leaves the tree keeps none of
-    its tokens and sets `STATUS_BAD_POSITION`.  `out` must not share memory with `seq_lens`."""
-    got = _lib.host().keep(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, counts, int(drafted), out,
-                           status)
+    its tokens and sets `STATUS_BAD_POSITION`.  `granted`: an int32 word that is 0 if the trees were refused
+    (the last of their plan's `starts`); nothing is kept or cut off then.  `out` must not share memory with `seq_lens`."""
+    got = _lib.host().keep(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, counts, int(drafted), granted,
+                           out, status)
     if got is not None:
         return got
     dev = _lib.require_cuda(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, counts)
@@ -316,6 +317,8 @@ def keep_tokens(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, 
             raise ValueError(f"{name} must be contiguous int32 ({B},)")
     if keep.dim() != 2 or keep.shape[0] != B or keep.dtype != torch.int32 or (keep.shape[1] > 1 and keep.stride(1) != 1):
         raise ValueError("keep must be int32 (B, A) with contiguous rows")
+    if granted is not None and (tuple(granted.shape) != (1,) or granted.dtype != torch.int32 or granted.device != dev):
+        raise ValueError("granted must be an int32 word on the pages' device")
     if out is None:
         out = torch.empty_like(seq_lens)
     if B and out.data_ptr() == seq_lens.data_ptr():
@@ -327,7 +330,8 @@ def keep_tokens(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, 
         _lib.check(_lib.lib().wtq_keep_tokens(
             ctypes.byref(sides[0]), ctypes.byref(sides[1]), page_table.data_ptr(), page_table.stride(0),
             seq_lens.data_ptr(), keep.data_ptr(), keep.stride(0), counts.data_ptr(), layers, B, Hkv, S, P,
-            page_table.shape[1], keep.shape[1], int(drafted), out.data_ptr(),
+            page_table.shape[1], keep.shape[1], int(drafted),
+            None if granted is None else granted.data_ptr(), out.data_ptr(),
             None if status is None else status.data_ptr(), _lib.stream_ptr(dev)))
     return out
 
