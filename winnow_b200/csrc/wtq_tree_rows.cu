@@ -146,6 +146,53 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms, 
       }
     }
   }
+  // Of joined states, first all that weights and addresses hang on, for all of a thread's rows at once: a row's
+  // pieces, a lane each, with maximum and sum (a whole group is one piece); then the first accumulators.
+  constexpr int kMine = JOIN ? kRows / kStep : 1, kAhead = 2;
+  int at_of[kMine] = {};                                         // state of its first piece; number e > 0 is (2 e - 1) * p.rows on
+  int n_of[kMine] = {};
+  float m_of[kMine], l_of[kMine];                           // of piece number `piece`
+  float4 ahead[kMine][kAhead][2];
+  auto fetch = [&](float4 (&to)[2], const float *from) {
+    to[0] = __ldcg(reinterpret_cast<const float4 *>(from));
+    to[1] = __ldcg(reinterpret_cast<const float4 *>(from) + 1);
+  };
+  auto state = [&](int k, int e) { return at_of[k] + (e ? (2 * e - 1) * p.rows : 0); };
+  auto acc = [&](int k, int e) { return (n_of[k] == 1 ? p.acc : p.part_acc) + (int64_t)state(k, e) * D + 8 * piece; };
+  if constexpr (JOIN) {
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      const int64_t row = row0 + first + k * kStep;
+      m_of[k] = -INFINITY;
+      l_of[k] = 0.f;
+      if (row >= rows) continue;
+      int b, i, h;
+      place(p, row, b, i, h);
+      const int n = prefix[b + 1] - prefix[b];
+      if (n == 0) continue;
+      const int kvh = h / p.n_rep, qr = i * p.n_rep + h - kvh * p.n_rep, rb = qr / p.rows;
+      const long long g0 = (long long)prefix[b] * p.row_blocks * p.Hkv + (long long)(rb * p.Hkv + kvh) * n;
+      const int c0 = run_of(g0, share);
+      n_of[k] = run_of(g0 + n - 1, share) - c0 + 1;
+      at_of[k] = n_of[k] == 1 ? (int)row : (c0 * 2 + 1) * p.rows + qr - rb * p.rows;
+      if (n_of[k] == 1) {
+        if (piece == 0) {
+          l_of[k] = __ldcg(p.l + row);
+          m_of[k] = l_of[k] != 0.f ? 0.f : -INFINITY;
+        }
+      } else if (piece < n_of[k]) {
+        m_of[k] = __ldcg(p.part_m + state(k, piece));
+        l_of[k] = __ldcg(p.part_l + state(k, piece));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kMine; ++k)
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) {
+        ahead[k][e][0] = ahead[k][e][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (e < n_of[k]) fetch(ahead[k][e], acc(k, e));
+      }
+  }
 #pragma unroll
   for (int k = 0; k < kRows / kStep; ++k) {
     const int r = first + k * kStep;
@@ -154,10 +201,10 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms, 
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = 0.f;
-    int b = 0, i = 0, h = 0;
-    if (row < rows) place(p, row, b, i, h);
     if constexpr (!JOIN) {
       if (row < rows && !wide) {
+        int b, i, h;
+        place(p, row, b, i, h);
         const int64_t at = b * p.qb + i * p.qt + h * p.qh + 8 * piece;
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = load_as_float(p.q, at + e, p.dtype);
@@ -177,36 +224,40 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms, 
         }
       }
     } else {
-      const int n = row < rows ? prefix[b + 1] - prefix[b] : 0;
-      const int kvh = h / p.n_rep, qr = i * p.n_rep + h - kvh * p.n_rep, rb = qr / p.rows;
-      const long long g0 = (long long)prefix[b] * p.row_blocks * p.Hkv + (long long)(rb * p.Hkv + kvh) * n;
-      const int c0 = n > 0 ? run_of(g0, share) : 0, c1 = n > 0 ? run_of(g0 + n - 1, share) : -1;
-      auto add = [&](const float *acc, float w) {
-        const float4 a = __ldcg(reinterpret_cast<const float4 *>(acc + 8 * piece));
-        const float4 c = __ldcg(reinterpret_cast<const float4 *>(acc + 8 * piece) + 1);
-        x[0] = fmaf(w, a.x, x[0]); x[1] = fmaf(w, a.y, x[1]); x[2] = fmaf(w, a.z, x[2]); x[3] = fmaf(w, a.w, x[3]);
-        x[4] = fmaf(w, c.x, x[4]); x[5] = fmaf(w, c.y, x[5]); x[6] = fmaf(w, c.z, x[6]); x[7] = fmaf(w, c.w, x[7]);
+      auto add = [&](const float4 (&v)[2], float w) {
+        x[0] = fmaf(w, v[0].x, x[0]); x[1] = fmaf(w, v[0].y, x[1]); x[2] = fmaf(w, v[0].z, x[2]); x[3] = fmaf(w, v[0].w, x[3]);
+        x[4] = fmaf(w, v[1].x, x[4]); x[5] = fmaf(w, v[1].y, x[5]); x[6] = fmaf(w, v[1].z, x[6]); x[7] = fmaf(w, v[1].w, x[7]);
       };
-      if (c0 == c1) {                                       // an empty state's accumulator is not read
-        const float l = p.l[row];
-        if (l != 0.f) add(p.acc + row * D, 1.f / l);
-      } else if (c0 < c1) {
-        // the row's lanes look at a piece each; then all add up its coordinates, piece by piece
-        auto state = [&](int c) -> int64_t { return ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * p.rows + qr - rb * p.rows; };
-        const uint32_t group = (kPieces == 32 ? 0xffffffffu : ((1u << kPieces) - 1u)) << (lane / kPieces * kPieces);
-        float top = -INFINITY, sum = 0.f;
-        for (int c = c0 + piece; c <= c1; c += kPieces) top = fmaxf(top, p.part_m[state(c)]);
+      const uint32_t group = (kPieces == 32 ? 0xffffffffu : ((1u << kPieces) - 1u)) << (lane / kPieces * kPieces);
+      const int n = n_of[k], lane0 = lane / kPieces * kPieces;
+      // A row with nothing to see has sum 0, and what its accumulators hold (they may never have been written) is not
+      // used; other rows' are all written.
+      if (n > 0) {
+        float top = m_of[k];
+        for (int e = piece + kPieces; e < n; e += kPieces) top = fmaxf(top, __ldcg(p.part_m + state(k, e)));
 #pragma unroll
         for (int o = kPieces / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(group, top, o));
-        for (int from = c0; from <= c1; from += kPieces) {
-          const int c = from + piece;
-          const float m = c <= c1 ? p.part_m[state(c)] : -INFINITY;
+        float m = m_of[k], l = l_of[k], sum = 0.f;
+        for (int from = 0; from < n; from += kPieces) {
+          if (from > 0) {
+            const int e = from + piece;
+            m = e < n ? __ldcg(p.part_m + state(k, e)) : -INFINITY;
+            l = e < n ? __ldcg(p.part_l + state(k, e)) : 0.f;
+          }
           const float w = m == -INFINITY ? 0.f : exp2f(m - top);
-          if (m != -INFINITY) sum = fmaf(w, p.part_l[state(c)], sum);   // (NaN counts whatever its weight)
-          const int last = min(kPieces, c1 - from + 1);
-#pragma unroll 8
-          for (int e = 0; e < last; ++e)                    // (a live row's accumulators are all written)
-            add(p.part_acc + state(from + e) * D, __shfl_sync(group, w, lane / kPieces * kPieces + e));
+          if (m != -INFINITY) sum = fmaf(w, l, sum);        // (NaN counts whatever its weight)
+          int e = from;
+          if (from == 0) {
+#pragma unroll
+            for (; e < kAhead; ++e) add(ahead[k][e], __shfl_sync(group, w, lane0 + e));
+          }
+          const int last = min(n, from + kPieces);
+#pragma unroll 4
+          for (; e < last; ++e) {
+            float4 v[2];
+            fetch(v, acc(k, e));
+            add(v, __shfl_sync(group, w, lane0 + e - from));
+          }
         }
 #pragma unroll
         for (int o = kPieces / 2; o; o >>= 1) sum += __shfl_xor_sync(group, sum, o);

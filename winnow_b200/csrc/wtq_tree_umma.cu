@@ -21,10 +21,10 @@
 // flag that ends all others, and the status word says so.
 //
 // A warp on its own gets through an instruction in about nine cycles here, so a role is only as fast
-// as its instructions per tile are few.  Bound by the chain of a stream's tile, scores ready to
-// probabilities stored, and by issue slots (4.1 K warp instructions a tile, 53 % of the slots used); the
-// tensor pipe is active a quarter of the time.  16 x 8 kv heads x 8192 tokens, 128 rows a group, 4 bits:
-// 119 us (69 GFLOP; 579 TFLOP/s), 8 x 131 072 tokens, 512 rows a group: 369 us (745 TFLOP/s).
+// as its instructions per tile are few and as they are in the instruction cache: the roles' hot loops
+// together are more than it holds, and a few dozen instructions more in any of them cost 5 to 25 %.  The tensor
+// pipe is active a quarter of the time.  16 x 8 kv heads x 8192 tokens, 128 rows a group, 4 bits (69 GFLOP): 146 us
+// with both rotations; 8 x 131 072 tokens, 512 rows a group (275 GFLOP): 374 us, 735 TFLOP/s.
 //
 // Rounded to fp16, because the products' operands are: query rows, centroids, centroid times norm and
 // probabilities; sums, maxima and states are fp32.  Measured on fp16 results against 64 bits: 8.2e-4 over
@@ -142,10 +142,31 @@ __device__ __forceinline__ uint32_t times(uint32_t c, __half2 n) {
   return *reinterpret_cast<const uint32_t *>(&y);
 }
 
-// One side's fetch warp: page ids of eight tiles ahead, a lane per 16 tokens.
+// A bit for each of the 16 fp16 numbers at `from` that is not finite.  Out of line: rarely called.
+__device__ __noinline__ uint32_t not_finite(const __half *from) {
+  uint32_t bad = 0;
+#pragma unroll 1
+  for (int i = 0; i < 16; ++i) bad |= (uint32_t)!(fabsf(__half2float(from[i])) < INFINITY) << i;
+  return bad;
+}
+// Whether sixteen fp16 numbers all give zero when multiplied with zero.
+__device__ __forceinline__ bool all_finite(const uint4 &a, const uint4 &b) {
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  const __half2 zero = __float2half2_rn(0.f);
+  __half2 t = zero;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t = __hfma2(*reinterpret_cast<const __half2 *>(&w[i]), zero, t);
+  return __hbeq2(t, zero);
+}
+
+// One side's fetch warp: page ids of eight tiles ahead, a lane per 16 tokens.  A value norm that is not finite
+// is replaced by zero, since the product would carry it (0 x inf) to rows that do not see its token;
+// those that do are found when the piece ends (spoiled()).  A look at a lane's norms every eight tiles does
+// it here; in the decode warps' loop the same check took 7 % of a long scan.
 template <int BW, int D, int RAW_TILES>
-__device__ __forceinline__ void fetch_role(const Params &p, const DecodeSideDev &sd, const int *prefix, long long begin,
-                                           long long end, int side, uint32_t ring) {
+__device__ __forceinline__ void fetch_role(const Params &p, int side, const int *prefix, long long begin, long long end,
+                                           uint32_t ring) {
+  const DecodeSideDev sd = side ? p.v : p.k;
   constexpr int kBytes = 16 * D * BW / 8;                   // codes of 16 tokens
   constexpr uint32_t kRawBytes = 4 * kBytes + 2 * kTile;
   const int lane = threadIdx.x & 31, page_shift = 31 - __clz(p.S);
@@ -164,8 +185,9 @@ __device__ __forceinline__ void fetch_role(const Params &p, const DecodeSideDev 
     int ahead = page_of(c.first);
     uint32_t from_lo = 0, from_hi = 0;                      // where this lane's 16 tokens' codes are
     const __half *norms_from = norms;
-    uint32_t norm_bytes = 0;                                // of this lane's 16 tokens, those that exist
+    uint32_t norm_bytes = 0, bad = 0;                       // of this lane's 16 tokens: those that exist; norms not finite
     bool good = false;
+    uint32_t goods = 0;
     for (int tile = c.first; tile < c.last; ++tile, raw.next()) {
       const int step = (tile - c.first) & 7;
       if (step == 0) {
@@ -178,24 +200,37 @@ __device__ __forceinline__ void fetch_role(const Params &p, const DecodeSideDev 
         from_hi = (uint32_t)(from >> 32);
         norms_from = good ? norms + (int64_t)page * sd.norm_page_stride + slot : norms;
         norm_bytes = good ? 2u * (uint32_t)min(16, L - (tile * kTile + 16 * lane)) : 0u;
+        goods = __ballot_sync(kFull, good);
+        bad = 0u;
+        if (good && side) {
+          const uint4 *n = reinterpret_cast<const uint4 *>(norms_from);
+          if (!all_finite(__ldg(n), __ldg(n + 1))) bad = not_finite(norms_from) & ((1u << (norm_bytes / 2)) - 1u);
+        }
+        if (bad != 0u) sts32(kBadNorm, 1u);
       }
       const uint32_t bar = (uint32_t)(side * kMostRaw + raw.at) * 8u, at = ring + (uint32_t)raw.at * kRawBytes;
       if (raw.use > 0 && !warp_wait(kRawFree + bar, raw.use - 1)) return;
-      const uint32_t goods = __ballot_sync(kFull, good) >> (4 * step);
+      const int owner = 4 * step + (lane >> 3);             // whose 16 tokens this lane copies an eighth of
+      const uint64_t lo = __shfl_sync(kFull, from_lo, owner), hi = __shfl_sync(kFull, from_hi, owner);
+      const uint32_t there = (goods >> owner & 1u) << 4;    // bytes of a copy
+      const uint8_t *from = (const uint8_t *)(lo | hi << 32) + (there ? 16 * (lane & 7) : 0);
+      const uint32_t to = at + (uint32_t)(lane >> 3) * kBytes + 16u * (lane & 7);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const uint64_t lo = __shfl_sync(kFull, from_lo, 4 * step + u), hi = __shfl_sync(kFull, from_hi, 4 * step + u);
-        const uint8_t *from = (const uint8_t *)(lo | hi << 32);
-        const uint32_t there = (goods >> u & 1u) << 4;      // bytes of a copy
-#pragma unroll
-        for (int e = 0; e < kBytes; e += 512)
-          if (kBytes - e >= 512 || 16 * lane < kBytes - e)
-            copy16(at + (uint32_t)(u * kBytes + e) + 16u * lane, from + (there ? e + 16 * lane : 0), there);
-      }
+      for (int e = 0; e < kBytes; e += 128) copy16(to + e, from + e, there);
       if (lane >> 2 == step) {                              // the lane that knows the page
         const uint32_t to = at + 4 * kBytes + 32u * (lane & 3);
-        copy16(to, norms_from, min(norm_bytes, 16u));
-        copy16(to + 16, norms_from + (good ? 8 : 0), norm_bytes > 16u ? norm_bytes - 16u : 0u);
+        if (bad != 0u) {
+#pragma unroll 1
+          for (uint32_t i = 0; i < 16; i += 2) {
+            auto kept = [&](uint32_t k) { return 2 * k < norm_bytes && !(bad >> k & 1u) ? norms_from[k] : __float2half(0.f); };
+            const __half2 two = __halves2half2(kept(i), kept(i + 1));
+            sts32(to + 2 * i, *reinterpret_cast<const uint32_t *>(&two));
+          }
+          __threadfence_block();
+        } else {
+          copy16(to, norms_from, min(norm_bytes, 16u));
+          copy16(to + 16, norms_from + (good ? 8 : 0), norm_bytes > 16u ? norm_bytes - 16u : 0u);
+        }
       }
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(kRawFull + bar) : "memory");
     }
@@ -203,12 +238,9 @@ __device__ __forceinline__ void fetch_role(const Params &p, const DecodeSideDev 
 }
 
 // One decode warp: its eight or sixteen tokens of every tile of a side, lane (g, t) rows g (and g + 8) of
-// them, coordinates t * D / 4 on.  A value row whose norm is not finite becomes zeros, since the
-// product would carry it (0 x inf) to rows that do not see its token; those that do are found when the
-// piece ends (spoiled()).
-template <int BW, int D, int RAW_TILES, bool VALUES>
-__device__ __forceinline__ void decode_role(int tiles, int u, uint32_t ring, uint32_t tile_base) {
-  constexpr int side = VALUES;
+// them, coordinates t * D / 4 on.
+template <int BW, int D, int RAW_TILES>
+__device__ __forceinline__ void decode_role(int tiles, int side, int u, uint32_t ring, uint32_t tile_base) {
   constexpr int kRowBytes = D * BW / 8, kPairs = D / 8;     // code pairs of a quarter
   constexpr int kGroups = 8 / decode_warps(BW);             // groups of eight tokens
   constexpr uint32_t kRawBytes = kTile * kRowBytes + 2 * kTile, kTileBytes = kTile * D * 2;
@@ -232,10 +264,6 @@ __device__ __forceinline__ void decode_role(int tiles, int u, uint32_t ring, uin
     for (int h = 0; h < kGroups; ++h) {
       load_words<kRowBytes / 4>(codes + off + (uint32_t)(8 * h * kRowBytes), w[h]);
       n[h] = __float2half2_rn(lds_half(norms + off + 16u * h));
-      if (VALUES && !__hlt(__habs(__low2half(n[h])), __ushort_as_half(0x7c00))) {
-        n[h] = __float2half2_rn(0.f);
-        sts32(kBadNorm, 1u);
-      }
     }
 #pragma unroll
     for (int h = 0; h < kGroups; ++h) {
@@ -581,11 +609,21 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D>::kThreads, 1) scan_kernel(con
     }
   } else if (warp < M::kFetch) {
     const int tiles = (int)max(0LL, end - begin);
-    if (warp < M::kDecodeV) decode_role<BWK, D, M::kRawTiles, false>(tiles, warp - M::kDecodeK, M::kRaw, M::kKTile);
-    else decode_role<BWV, D, M::kRawTiles, true>(tiles, warp - M::kDecodeV, M::kRaw + M::kRawTiles * M::kRawK, kVTile);
+    // Sides of one width run the same instructions, as these are what the roles share least of: the block's
+    // hot loops are more than the instruction cache holds (it hit 89 %, and the next level was at 77 % of its
+    // rate): 16 x 8 k 154 -> 146 us, 1 x 128 k 397 -> 374 us.
+    if constexpr (BWK == BWV) {
+      const bool v = warp >= M::kDecodeV;
+      decode_role<BWK, D, M::kRawTiles>(tiles, v, warp - (v ? M::kDecodeV : M::kDecodeK),
+                                        M::kRaw + (v ? M::kRawTiles * M::kRawK : 0u), v ? kVTile : M::kKTile);
+    } else if (warp < M::kDecodeV) decode_role<BWK, D, M::kRawTiles>(tiles, 0, warp - M::kDecodeK, M::kRaw, M::kKTile);
+    else decode_role<BWV, D, M::kRawTiles>(tiles, 1, warp - M::kDecodeV, M::kRaw + M::kRawTiles * M::kRawK, kVTile);
   } else if (warp < M::kScore) {
-    if (warp == M::kFetch) fetch_role<BWK, D, M::kRawTiles>(p, p.k, prefix, begin, end, 0, M::kRaw);
-    else fetch_role<BWV, D, M::kRawTiles>(p, p.v, prefix, begin, end, 1, M::kRaw + M::kRawTiles * M::kRawK);
+    if constexpr (BWK == BWV) {
+      const bool v = warp != M::kFetch;
+      fetch_role<BWK, D, M::kRawTiles>(p, v, prefix, begin, end, M::kRaw + (v ? M::kRawTiles * M::kRawK : 0u));
+    } else if (warp == M::kFetch) fetch_role<BWK, D, M::kRawTiles>(p, 0, prefix, begin, end, M::kRaw);
+    else fetch_role<BWV, D, M::kRawTiles>(p, 1, prefix, begin, end, M::kRaw + M::kRawTiles * M::kRawK);
     asm volatile("cp.async.wait_all;\n" ::: "memory");     // (a block that gave up leaves no copies behind)
   } else {
     // ================= multiply: one lane issues ===========================================
