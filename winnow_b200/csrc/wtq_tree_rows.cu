@@ -9,7 +9,7 @@
 // element first, and Pi by 2^8, so that low parts stay clear of fp16's subnormal range.  Pi is laid out
 // as the operand once and serves both: read along its rows for the queries (K-major), across them for
 // the states (MN-major).  A thread per row quarter converts and stores.  Bound by the reads of rows and of
-// Pi from L2: 13 and 26 us from a cold cache at 16 384 rows, where the CUDA-core kernels of wtq_tree.cu
+// Pi from L2: about 13 and 20 us from a cold cache at 16 384 rows, where the CUDA-core kernels of wtq_tree.cu
 // take 187 and 70.
 #include <algorithm>
 #include <atomic>
@@ -81,8 +81,8 @@ __device__ __forceinline__ int run_of(long long x, long long share) {
   return ((x | share) >> 31) == 0 ? (int)((uint32_t)x / (uint32_t)share) : (int)(x / share);
 }
 
-template <bool JOIN, int D>
-__global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms, int rows_per) {
+template <bool JOIN, int D, bool WIDE>
+__global__ void __launch_bounds__(kThreads, WIDE ? 1 : 2) product_kernel(Params p, int terms, int rows_per) {
   using M = Map<D>;
   extern __shared__ __align__(1024) uint8_t dyn_smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -146,9 +146,9 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms, 
       }
     }
   }
-  // Of joined states, first all that weights and addresses hang on, for all of a thread's rows at once: a row's
+  // Of joined states, first all that weights and addresses hang on, for several of a thread's rows at once: a row's
   // pieces, a lane each, with maximum and sum (a whole group is one piece); then the first accumulators.
-  constexpr int kMine = JOIN ? kRows / kStep : 1, kAhead = 2;
+  constexpr int kMine = !JOIN ? 1 : WIDE ? kRows / kStep : 2, kAhead = WIDE ? 2 : 1;
   int at_of[kMine] = {};                                         // state of its first piece; number e > 0 is (2 e - 1) * p.rows on
   int n_of[kMine] = {};
   float m_of[kMine], l_of[kMine];                           // of piece number `piece`
@@ -159,10 +159,11 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms, 
   };
   auto state = [&](int k, int e) { return at_of[k] + (e ? (2 * e - 1) * p.rows : 0); };
   auto acc = [&](int k, int e) { return (n_of[k] == 1 ? p.acc : p.part_acc) + (int64_t)state(k, e) * D + 8 * piece; };
-  if constexpr (JOIN) {
+  auto read_ahead = [&](int from_row) {
 #pragma unroll
     for (int k = 0; k < kMine; ++k) {
-      const int64_t row = row0 + first + k * kStep;
+      const int64_t row = row0 + from_row + k * kStep;
+      n_of[k] = 0;
       m_of[k] = -INFINITY;
       l_of[k] = 0.f;
       if (row >= rows) continue;
@@ -192,12 +193,14 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms, 
         ahead[k][e][0] = ahead[k][e][1] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (e < n_of[k]) fetch(ahead[k][e], acc(k, e));
       }
-  }
+  };
 #pragma unroll
   for (int k = 0; k < kRows / kStep; ++k) {
     const int r = first + k * kStep;
     if (k > 0 && k * kStep >= rows_per) break;              // (the same for all)
     const int64_t row = row0 + r;
+    if constexpr (JOIN)
+      if (k % kMine == 0) read_ahead(r);
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = 0.f;
@@ -224,38 +227,39 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms, 
         }
       }
     } else {
+      const int at = k % kMine;
       auto add = [&](const float4 (&v)[2], float w) {
         x[0] = fmaf(w, v[0].x, x[0]); x[1] = fmaf(w, v[0].y, x[1]); x[2] = fmaf(w, v[0].z, x[2]); x[3] = fmaf(w, v[0].w, x[3]);
         x[4] = fmaf(w, v[1].x, x[4]); x[5] = fmaf(w, v[1].y, x[5]); x[6] = fmaf(w, v[1].z, x[6]); x[7] = fmaf(w, v[1].w, x[7]);
       };
       const uint32_t group = (kPieces == 32 ? 0xffffffffu : ((1u << kPieces) - 1u)) << (lane / kPieces * kPieces);
-      const int n = n_of[k], lane0 = lane / kPieces * kPieces;
+      const int n = n_of[at], lane0 = lane / kPieces * kPieces;
       // A row with nothing to see has sum 0, and what its accumulators hold (they may never have been written) is not
       // used; other rows' are all written.
       if (n > 0) {
-        float top = m_of[k];
-        for (int e = piece + kPieces; e < n; e += kPieces) top = fmaxf(top, __ldcg(p.part_m + state(k, e)));
+        float top = m_of[at];
+        for (int e = piece + kPieces; e < n; e += kPieces) top = fmaxf(top, __ldcg(p.part_m + state(at, e)));
 #pragma unroll
         for (int o = kPieces / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(group, top, o));
-        float m = m_of[k], l = l_of[k], sum = 0.f;
+        float m = m_of[at], l = l_of[at], sum = 0.f;
         for (int from = 0; from < n; from += kPieces) {
           if (from > 0) {
             const int e = from + piece;
-            m = e < n ? __ldcg(p.part_m + state(k, e)) : -INFINITY;
-            l = e < n ? __ldcg(p.part_l + state(k, e)) : 0.f;
+            m = e < n ? __ldcg(p.part_m + state(at, e)) : -INFINITY;
+            l = e < n ? __ldcg(p.part_l + state(at, e)) : 0.f;
           }
           const float w = m == -INFINITY ? 0.f : exp2f(m - top);
           if (m != -INFINITY) sum = fmaf(w, l, sum);        // (NaN counts whatever its weight)
           int e = from;
           if (from == 0) {
 #pragma unroll
-            for (; e < kAhead; ++e) add(ahead[k][e], __shfl_sync(group, w, lane0 + e));
+            for (; e < kAhead; ++e) add(ahead[at][e], __shfl_sync(group, w, lane0 + e));
           }
           const int last = min(n, from + kPieces);
 #pragma unroll 4
           for (; e < last; ++e) {
             float4 v[2];
-            fetch(v, acc(k, e));
+            fetch(v, acc(at, e));
             add(v, __shfl_sync(group, w, lane0 + e - from));
           }
         }
@@ -353,29 +357,38 @@ __global__ void __launch_bounds__(kThreads) product_kernel(Params p, int terms, 
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"((uint32_t)D) : "memory");
 }
 
-template <bool JOIN, int D> int launch(const Params &p, cudaStream_t stream) {
+template <bool JOIN, int D, bool WIDE> int launch_blocks(const Params &p, int rows_per, int blocks, cudaStream_t stream) {
   using M = Map<D>;
   static std::atomic<bool> opted_in[64];
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 64 || !opted_in[dev & 63].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(product_kernel<JOIN, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    const cudaError_t e = cudaFuncSetAttribute(product_kernel<JOIN, D, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (int)M::kBytes);
     if (e != cudaSuccess) return check_cuda(e, "wtq_tree: shared memory opt-in");
     opted_in[dev & 63].store(true, std::memory_order_release);
   }
+  const int terms = p.dtype == WTQ_F32 || (JOIN && p.dtype == WTQ_F16) ? 3 : 2;
+  const size_t bytes = terms > 2 ? M::kBytes : M::kALow;    // (two blocks a multiprocessor without low parts)
+  if (JOIN)
+    return launch_behind(product_kernel<JOIN, D, WIDE>, blocks, kThreads, bytes, stream, "wtq_tree join launch", p, terms, rows_per);
+  product_kernel<JOIN, D, WIDE><<<blocks, kThreads, bytes, stream>>>(p, terms, rows_per);
+  note_launches(1);
+  return check_cuda(cudaGetLastError(), "wtq_tree rotate launch");
+}
+template <bool JOIN, int D> int launch(const Params &p, cudaStream_t stream) {
   const int64_t all = (int64_t)p.B * p.Q * p.Hq;
   // Few rows are spread over more blocks, as far as there are multiprocessors: a block's time is the
   // chain of reads that its rows' pieces make (2688 rows of 8 pieces: 26 us on 21 blocks).
   int rows_per = kRows;
   while (rows_per > 16 && (all + rows_per / 2 - 1) / (rows_per / 2) <= device_sms()) rows_per /= 2;
-  const int blocks = (int)((all + rows_per - 1) / rows_per), terms = p.dtype == WTQ_F32 || (JOIN && p.dtype == WTQ_F16) ? 3 : 2;
-  const size_t bytes = terms > 2 ? M::kBytes : M::kALow;    // (two blocks a multiprocessor without low parts)
-  if (JOIN)
-    return launch_behind(product_kernel<JOIN, D>, blocks, kThreads, bytes, stream, "wtq_tree join launch", p, terms, rows_per);
-  product_kernel<JOIN, D><<<blocks, kThreads, bytes, stream>>>(p, terms, rows_per);
-  note_launches(1);
-  return check_cuda(cudaGetLastError(), "wtq_tree rotate launch");
+  const int blocks = (int)((all + rows_per - 1) / rows_per);
+  // A join that has a multiprocessor for every block reads all of a thread's rows ahead, in up to 128 registers
+  // (16 384 rows: call 151 -> 146 us); more blocks than that are better off two a multiprocessor (19 968 rows:
+  // 320 -> 307 us).
+  if constexpr (JOIN)
+    if (blocks <= device_sms()) return launch_blocks<true, D, true>(p, rows_per, blocks, stream);
+  return launch_blocks<JOIN, D, false>(p, rows_per, blocks, stream);
 }
 
 }  // namespace rows
