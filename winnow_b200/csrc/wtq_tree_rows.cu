@@ -9,7 +9,7 @@
 // element first, and Pi by 2^8, so that low parts stay clear of fp16's subnormal range.  Pi is laid out
 // as the operand once and serves both: read along its rows for the queries (K-major), across them for
 // the states (MN-major).  A thread per row quarter converts and stores.  Bound by the reads of rows and of
-// Pi from L2: about 13 and 20 us from a cold cache at 16 384 rows, where the CUDA-core kernels of wtq_tree.cu
+// Pi from L2: 13 and 21 us from a cold cache at 16 384 rows, where the CUDA-core kernels of wtq_tree.cu
 // take 187 and 70.
 #include <algorithm>
 #include <atomic>

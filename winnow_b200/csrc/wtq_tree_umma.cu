@@ -21,9 +21,10 @@
 // flag that ends all others, and the status word says so.
 //
 // A warp on its own gets through an instruction in about nine cycles here, so a role is only as fast
-// as its instructions per tile are few and as they are in the instruction cache: the roles' hot loops
-// together are more than it holds, and a few dozen instructions more in any of them cost 5 to 25 %.  The tensor
-// pipe is active a quarter of the time.  16 x 8 kv heads x 8192 tokens, 128 rows a group, 4 bits (69 GFLOP): 146 us
+// as its instructions per tile are few and lie in the instruction cache: with code of its own for each side
+// the roles' loops were more than that holds (hit rate 89 %, the level behind at 77 % of its rate), and a
+// few dozen instructions more cost 5 to 25 %.  Now (98 %, 30 %) bound by the chain of a stream's tile, scores ready
+// to probabilities stored; issue slots 46 % used, the tensor pipe active 29 % of the time.  16 x 8 kv heads x 8192 tokens, 128 rows a group, 4 bits (69 GFLOP): 146 us
 // with both rotations; 8 x 131 072 tokens, 512 rows a group (275 GFLOP): 374 us, 735 TFLOP/s.
 //
 // Rounded to fp16, because the products' operands are: query rows, centroids, centroid times norm and
@@ -609,9 +610,8 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D>::kThreads, 1) scan_kernel(con
     }
   } else if (warp < M::kFetch) {
     const int tiles = (int)max(0LL, end - begin);
-    // Sides of one width run the same instructions, as these are what the roles share least of: the block's
-    // hot loops are more than the instruction cache holds (it hit 89 %, and the next level was at 77 % of its
-    // rate): 16 x 8 k 154 -> 146 us, 1 x 128 k 397 -> 374 us.
+    // Sides of one width run the same instructions, for the instruction cache's sake: 16 x 8 k 152 -> 145 us
+    // (with the fetch warps' shorter loop), 1 x 128 k 397 -> 373 us.
     if constexpr (BWK == BWV) {
       const bool v = warp >= M::kDecodeV;
       decode_role<BWK, D, M::kRawTiles>(tiles, v, warp - (v ? M::kDecodeV : M::kDecodeK),
