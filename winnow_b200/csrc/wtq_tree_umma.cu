@@ -65,9 +65,9 @@ constexpr uint32_t kSFull = kRawFree + 16 * kMostRaw, kSFree = kSFull + 16, kPFu
 constexpr uint32_t kQFull = kODone + 16, kLast = kQFull + 8, kTmemSlot = kLast + 8, kAbort = kTmemSlot + 4,
                    kBadNorm = kAbort + 4;                                  // a value norm that is not finite was met
 constexpr uint32_t kPrefix = kBase + 512;                                  // kMaxBatch + 1 words
-constexpr uint32_t kStates = kPrefix + 4 * (kMaxBatch + 4);                // [stream][m, l][row]
+constexpr uint32_t kStates = kPrefix + 4 * (kMaxBatch + 4);                // [piece's parity][stream][m, l][row]
 constexpr uint32_t kVTile = 16384;
-static_assert(kBadNorm + 4 <= kPrefix && kStates + 4 * kRows * 4 <= kVTile, "low region");
+static_assert(kBadNorm + 4 <= kPrefix && kStates + 2 * 4 * kRows * 4 <= kVTile, "low region");
 static_assert(kVTile + kStages * kTile * 256 <= mma::kLutAddr, "value tiles end where the tables begin");
 // tensor memory columns
 constexpr uint32_t kColQ = 0, kColS = 64, kColP = 192, kColO = 256, kCols = 512;   // S + 64, P + 32, O + 128 per stream
@@ -445,6 +445,8 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D>::kThreads, 1) scan_kernel(con
     const uint32_t s_addr = tmem + lanes + kColS + 64u * st, p_addr = tmem + lanes + kColP + 32u * st,
                    o_addr = tmem + lanes + kColO + 128u * st;
     int n = 0;                                              // units of this stream so far
+    uint32_t states = kStates + 4u * r;                     // of this row, in the present piece's copy
+    bool piece_odd = false;
     bool ok = true;
     asm volatile("griddepcontrol.wait;\n" ::: "memory");   // the rotated queries (all else is there already)
     for (long long x = begin; x < end;) {
@@ -562,14 +564,16 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D>::kThreads, 1) scan_kernel(con
       }
       // ---- the rows' states: the two streams joined, half of the coordinates to each warpgroup ----
       if (ok && mine > 0) ok = warp_wait(kODone + 8u * st, n - 1);
-      sts32(kStates + 4u * ((2 * st) * kRows + r), __float_as_uint(ref));
-      sts32(kStates + 4u * ((2 * st + 1) * kRows + r), __float_as_uint(sum));
+      // (two copies, by turns: a stream without a tile in the next piece waits for nothing in it, and may write its
+      // state there while the other still reads this one; the barrier below keeps it from going a piece further)
+      sts32(states + 4u * ((2 * st) * kRows), __float_as_uint(ref));
+      sts32(states + 4u * ((2 * st + 1) * kRows), __float_as_uint(sum));
       fence_before();
       asm volatile("bar.sync 1, %0;\n" ::"r"(32 * kSoftWarps) : "memory");   // every softmax warp, whatever it gave up on
       fence_after();
       ok = __all_sync(kFull, ok && lds32(kAbort) == 0u);
       if (ok) {
-        auto state = [&](int what) { return __uint_as_float(lds32(kStates + 4u * (what * kRows + r))); };
+        auto state = [&](int what) { return __uint_as_float(lds32(states + 4u * (what * kRows))); };
         const float m0 = state(0), m1 = state(2);
         float top = fmaxf(m0, m1);
         const float l0 = state(1), l1 = state(3);
@@ -607,6 +611,8 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D>::kThreads, 1) scan_kernel(con
           }
         }
       }
+      states += piece_odd ? 0u - 16u * kRows : 16u * kRows;
+      piece_odd = !piece_odd;
     }
   } else if (warp < M::kFetch) {
     const int tiles = (int)max(0LL, end - begin);
