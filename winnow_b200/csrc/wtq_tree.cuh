@@ -14,7 +14,7 @@
 namespace wtq {
 namespace tree {
 
-constexpr int kMaxBatch = 2048;           // sequences of one launch (their tile prefix in shared memory)
+constexpr int kMaxBatch = 1024;           // sequences of one launch (their tile prefix in shared memory)
 
 struct Params {
   DecodeSideDev k, v;
