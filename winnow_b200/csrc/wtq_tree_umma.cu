@@ -638,9 +638,11 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D, VLOW>::kThreads, 1) scan_kern
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           const float2 y = halves(add2(pair(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), base));
-          const float a = ex2(y.x), b = ex2(y.y);
-          sums[e & 1] = add2(sums[e & 1], pair(a, b));
-          pr[e] = pack_half2(a, b);
+          pr[e] = pack_half2(ex2(y.x), ex2(y.y));
+          // The sum takes the probabilities as the product has them: where a few tokens carry the row, their
+          // rounding then cancels in the quotient.
+          const float2 rounded = __half22float2(as_half2(pr[e]));
+          sums[e & 1] = add2(sums[e & 1], pair(rounded.x, rounded.y));
         }
         const float2 both = halves(add2(sums[0], sums[1]));
         sum += both.x + both.y;
