@@ -359,7 +359,8 @@ int wtq_tree_on_tensor_cores(const wtq_side_t *k_side, const wtq_side_t *v_side,
 
 /* The accepted tokens of a tree stay: of the last `drafted` tokens of sequence b, token keep[b][i] becomes
  * token i for i < counts[b] (keep ascends; (B, most), row stride in elements), in every layer, as the
- * codes and norms it has; out[b] = seq_lens[b] - drafted + counts[b].  out must not be seq_lens.  A path
+ * codes and norms it has; out[b] = seq_lens[b] - drafted + counts[b].  out must not share memory with seq_lens,
+ * counts, keep, page_table or granted, which other blocks still read.  A path
  * that does not ascend or leaves the tree keeps nothing of it (out[b] = seq_lens[b] - drafted; where that
  * is negative, seq_lens[b]) and sets WTQ_STATUS_BAD_POSITION.  `granted` may be null; else it is a word
  * that is 0 if the trees were refused (starts[B] of their plan): nothing is kept or cut off then, out =

@@ -217,6 +217,18 @@ def reachable(what: str, t: torch.Tensor | None) -> None:
         raise BackendError(f"{what} is in pageable host memory, which the kernels cannot reach")
 
 
+def overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors' address ranges meet."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+
+    def span(t):
+        low = t.data_ptr()
+        return low, low + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 

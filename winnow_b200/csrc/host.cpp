@@ -594,8 +594,11 @@ PyObject *keep(PyObject *, PyObject *const *a, Py_ssize_t n) {
   }
   if (!words(lens, dev, {B}) || !words(counts, dev, {B}) || path.dim() != 2 || path.size(0) != B || path.size(1) < 1 ||
       path.stride(1) != 1 || path.scalar_type() != at::kInt || path.device() != dev ||
-      (out.defined() && (!words(out, dev, {B}) || out.storage().data() == lens.storage().data())))
+      (out.defined() && !words(out, dev, {B})))
     Py_RETURN_NONE;
+  if (out.defined())                      // memory of its own, else the Python path looks closer
+    for (const at::Tensor *t : {&table, &lens, &path, &counts, &granted})
+      if (t->defined() && out.storage().data() == t->storage().data()) Py_RETURN_NONE;
   const c10::cuda::OptionalCUDAGuard guard(dev);
   if (!out.defined()) out = at::empty({B}, lens.options());
   void *stream = (void *)at::cuda::getCurrentCUDAStream(dev.index()).stream();

@@ -25,6 +25,16 @@ void profile_mark_begin(cudaStream_t stream);
 void profile_mark_end(cudaStream_t stream);
 void profile_mark_call(cudaStream_t stream, bool begin);
 
+// Memory that a call reads or writes, for refusing calls whose results would lie over what is still read.
+struct Span {
+  const void *at;
+  int64_t bytes;
+};
+inline bool meet(const Span &a, const Span &b) {
+  const uintptr_t x = (uintptr_t)a.at, y = (uintptr_t)b.at;
+  return x && y && a.bytes > 0 && b.bytes > 0 && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
+}
+
 inline bool width_supported(int bw) {
   return bw == 2 || bw == 3 || bw == 4 || bw == 5 || bw == 6 || bw == 8;
 }

@@ -145,7 +145,13 @@ extern "C" int wtq_keep_tokens(const wtq_pool_side_t *k_side, const wtq_pool_sid
   if (B == 0) return WTQ_OK;
   if (!page_table || !seq_lens || !counts || !out || (most > 0 && !keep))
     return fail(WTQ_ERR_ARG, "wtq_keep_tokens: null argument");
-  if (out == seq_lens) return fail(WTQ_ERR_ARG, "wtq_keep_tokens: out must not be seq_lens");
+  // (one warp writes a sequence's result while those of its other layers, sides and heads read these)
+  const Span result = {out, (int64_t)B * 4};
+  const Span read[5] = {{seq_lens, (int64_t)B * 4}, {counts, (int64_t)B * 4}, {granted, 4},
+                        {keep, most > 0 ? ((B - 1) * keep_stride + most) * 4 : 0},
+                        {page_table, ((B - 1) * table_stride + max_pages) * 4}};
+  for (const Span &r : read)
+    if (meet(result, r)) return fail(WTQ_ERR_ARG, "wtq_keep_tokens: out must not share memory with what is read");
   keep::Params p = {};
   bool by16 = true, by4 = true;
   const wtq_pool_side_t *sides[2] = {k_side, v_side};

@@ -294,7 +294,8 @@ def keep_tokens(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, 
     (B, W), seq_lens (B,), counts (B,) and keep (B, A) int32, each row of keep ascending (what follows
     its counts[b] entries is not read).  A row that does not ascend or leaves the tree keeps none of
     its tokens and sets `STATUS_BAD_POSITION`.  `granted`: an int32 word that is 0 if the trees were refused
-    (the last of their plan's `starts`); nothing is kept or cut off then.  `out` must not share memory with `seq_lens`."""
+    (the last of their plan's `starts`); nothing is kept or cut off then.  `out` must not share memory with
+    any of the tensors that are read."""
     got = _lib.host().keep(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, counts, int(drafted), granted,
                            out, status)
     if got is not None:
@@ -321,8 +322,10 @@ def keep_tokens(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, 
         raise ValueError("granted must be an int32 word on the pages' device")
     if out is None:
         out = torch.empty_like(seq_lens)
-    if B and out.data_ptr() == seq_lens.data_ptr():
-        raise ValueError("out must not share memory with seq_lens")
+    for name, t in (("seq_lens", seq_lens), ("counts", counts), ("keep", keep), ("page_table", page_table),
+                    ("granted", granted)):
+        if t is not None and _lib.overlaps(out, t):      # (read while a sequence's result is written already)
+            raise ValueError(f"out must not share memory with {name}")
     layers, P, Hkv, S, _ = k_pages.shape
     sides = [_lib.PoolSide(pages.data_ptr(), norms.data_ptr(), *pages.stride()[:3], *norms.stride()[:3],
                            pages.shape[4]) for pages, norms in ((k_pages, k_norms), (v_pages, v_norms))]

@@ -50,18 +50,6 @@ def rotary_table(rot: int, positions: int, *, base: float = 10000.0, inv_freq: t
     return (torch.cat([angle.cos(), angle.sin()], -1) * scale).float().contiguous()
 
 
-def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two tensors' address ranges meet."""
-    if a.numel() == 0 or b.numel() == 0:
-        return False
-
-    def span(t):
-        low = t.data_ptr()
-        return low, low + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
-
-
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, *,
                  q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
                  interleaved: bool = False, v: torch.Tensor | None = None, out=None,
@@ -116,9 +104,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
         for i, o in enumerate(outs):
             for j, t in enumerate(xs):
                 same = i == j and o.data_ptr() == t.data_ptr() and o.stride() == t.stride()
-                if not same and _overlaps(o, t) and not _interleaved_slices(o, t):
+                if not same and _lib.overlaps(o, t) and not _interleaved_slices(o, t):
                     raise ValueError("out may be the inputs themselves, but must not overlap them in another way")
-            if any(_overlaps(o, t) and not _interleaved_slices(o, t) for t in outs[:i]):
+            if any(_lib.overlaps(o, t) and not _interleaved_slices(o, t) for t in outs[:i]):
                 raise ValueError("the tensors of out must not overlap")
     sides = (_lib.RopeSide * 3)()
     for i, (x, o) in enumerate(zip(xs, outs)):
