@@ -321,8 +321,9 @@ int wtq_qk_norm_rope(const wtq_rope_side_t sides[3], int dtype, int weight_dtype
  * Entries past the last token read -1 (slot_ends 0).  A step that the free pages or the table's width do
  * not cover is refused as a whole: no page is taken, seq_lens = lengths, every token entry is -1, the
  * masks are 0, and WTQ_STATUS_NO_PAGES is set (WTQ_STATUS_BAD_POSITION for negative numbers or more new
- * tokens than `tokens`).  State outputs may be the inputs; then `ticket`, a device word that is zero
- * between calls, must be given.  B <= 4096. */
+ * tokens than `tokens`).  State outputs may be the inputs that they advance; then `ticket`, a device word that is
+ * zero between calls, must be given.  Otherwise outputs and the table share memory neither with inputs nor with one
+ * another.  B <= 4096. */
 typedef struct {
   int32_t *seq_lens, *held, *free_count, *starts, *sequence, *positions, *slot_pages, *slot_ends, *mask;
 } wtq_plan_t;

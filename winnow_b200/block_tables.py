@@ -52,7 +52,7 @@ def plan_tokens(lengths, new_tokens, table, held, free_pages, free_count, page_s
     the table's width do not cover takes nothing and sets `STATUS_NO_PAGES` in `status`.
 
     The state comes back as new tensors, or goes to those of `out`; those may be the inputs
-    (lengths as seq_lens, held, free_count), with `ticket`, an int32 word that is zero.
+    (lengths as seq_lens, held, free_count), with `ticket`, an int32 word that is zero, and share no memory otherwise.
     """
     tree = parents is not None
     if tree == (new_tokens is not None):

@@ -266,6 +266,22 @@ extern "C" int wtq_plan_tokens(const int32_t *lengths, const int32_t *new_tokens
     return fail(WTQ_ERR_ARG, "wtq_plan_tokens: null token output");
   const bool in_place = out->seq_lens == lengths || out->held == held || out->free_count == free_count;
   if (in_place && !ticket) return fail(WTQ_ERR_ARG, "wtq_plan_tokens: state advanced in place needs a ticket word");
+  // Every block reads the inputs for itself while others write their results already: these lie apart from them and from
+  // one another, but for state that is advanced in place.
+  const int64_t n = tokens, words = parents ? (drafted + 31) / 32 : 0;
+  const Span read[6] = {{lengths, B * 4LL}, {held, B * 4LL}, {free_count, 4}, {parents ? nullptr : new_tokens, B * 4LL},
+                        {parents, parents ? ((B - 1) * parent_stride + drafted) * 4 : 0}, {free_pages, stack * 4LL}};
+  const Span written[11] = {{out->seq_lens, B * 4LL}, {out->held, B * 4LL}, {out->free_count, 4}, {out->starts, (B + 1) * 4LL},
+                            {out->sequence, n * 4}, {out->positions, n * 4}, {out->slot_pages, n * 4}, {out->slot_ends, n * 4},
+                            {parents ? out->mask : nullptr, n * words * 4}, {in_place ? ticket : nullptr, 4},
+                            {table, ((B - 1) * table_stride + max_pages) * 4}};
+  for (int i = 0; i < 11; ++i) {
+    for (int j = 0; j < 6; ++j)
+      if (!(i == j && i < 3 && written[i].at == read[j].at) && meet(written[i], read[j]))
+        return fail(WTQ_ERR_ARG, "wtq_plan_tokens: results must not share memory with inputs, but for their own state");
+    for (int j = 0; j < i; ++j)
+      if (meet(written[i], written[j])) return fail(WTQ_ERR_ARG, "wtq_plan_tokens: results must not share memory");
+  }
   plan::Params p = {lengths, new_tokens, parents, parent_stride, table, table_stride, held, free_pages, free_count,
                     B, max_pages, S, tokens, drafted, stack, out->seq_lens, out->held, out->free_count, out->starts,
                     out->sequence, out->positions, out->slot_pages, out->slot_ends, out->mask,
