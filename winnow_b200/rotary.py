@@ -63,7 +63,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     coordinates past rot are not turned.  Pairs are (i, i + rot / 2), or (2 i, 2 i + 1) with
     `interleaved`.  A side with a weight (D,) is divided by the root of its mean square (plus `eps`) and
     multiplied by the weight first.  With `v` the values are copied along and the result has three
-    tensors.  `out`: tensors of the same shapes to write into; they may be the inputs themselves.
+    tensors.  `out`: tensors of the same shapes to write into; they may be the inputs themselves, unless those
+    are broadcast.
     """
     got = _lib.host().rope(q, k, v, positions, table, q_weight, k_weight, float(eps), interleaved,
                            out if out is None else tuple(out), status)      # checked and launched in native code
@@ -101,6 +102,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
         if len(outs) != len(xs) or any(o.shape != t.shape or o.dtype != t.dtype or o.device != dev
                                        or (o.stride(-1) != 1 and D > 1) for o, t in zip(outs, xs)):
             raise ValueError("out needs a tensor of each input's shape and dtype with a contiguous last dimension")
+        if any(_meets_itself(o) for o in outs):            # (several blocks would write, or turn in place, the same memory)
+            raise ValueError("the tensors of out must not overlap themselves")
         for i, o in enumerate(outs):
             for j, t in enumerate(xs):
                 same = i == j and o.data_ptr() == t.data_ptr() and o.stride() == t.stride()
@@ -119,6 +122,16 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
             positions.stride(0), table.data_ptr(), table.stride(0), table.shape[0], B, n, D, table.shape[1],
             int(bool(interleaved)), None if status is None else status.data_ptr(), _lib.stream_ptr(dev)))
     return tuple(outs)
+
+
+def _meets_itself(t: torch.Tensor) -> bool:
+    """Whether two places of a tensor are one element, as in a broadcast one (strides that nest do not meet)."""
+    reach = 1
+    for step, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if step < reach:
+            return t.numel() > 0
+        reach = step * (n - 1) + reach
+    return False
 
 
 def _interleaved_slices(a: torch.Tensor, b: torch.Tensor) -> bool:
