@@ -217,6 +217,12 @@ def reachable(what: str, t: torch.Tensor | None) -> None:
         raise BackendError(f"{what} is in pageable host memory, which the kernels cannot reach")
 
 
+def no_tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    """Refuse tensors of forward-mode differentiation, whose tangents the result would drop in silence."""
+    if any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no derivatives: call it on tensors without tangents")
+
+
 def overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two tensors' address ranges meet."""
     if a.numel() == 0 or b.numel() == 0:

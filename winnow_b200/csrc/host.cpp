@@ -330,7 +330,10 @@ PyObject *stage(PyObject *, PyObject *const *a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-bool needs_grad(const at::Tensor &t) { return t.defined() && t.requires_grad() && c10::GradMode::is_enabled(); }
+// (a tangent of forward-mode differentiation is there whatever the mode of the backward one)
+bool needs_grad(const at::Tensor &t) {
+  return t.defined() && ((t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined());
+}
 bool optional(PyObject *o, at::Tensor &t) { return o == Py_None || tensor(o, t); }
 bool words(const at::Tensor &t, const at::Device &dev, at::IntArrayRef shape) {
   return t.scalar_type() == at::kInt && t.device() == dev && t.sizes() == shape && t.is_contiguous();
@@ -389,7 +392,7 @@ PyObject *rope(PyObject *, PyObject *const *a, Py_ssize_t n) {
     if (weight_dtype < 0 || (w[0].defined() && w[i].scalar_type() != w[0].scalar_type())) Py_RETURN_NONE;
   }
   if (positions.dim() != 2 || positions.size(0) != B || positions.size(1) != tokens || positions.stride(1) != 1 ||
-      positions.scalar_type() != at::kInt || positions.device() != dev || table.dim() != 2 || table.stride(1) != 1 ||
+      positions.scalar_type() != at::kInt || positions.device() != dev || needs_grad(table) || table.dim() != 2 || table.stride(1) != 1 ||
       table.scalar_type() != at::kFloat || table.device() != dev || table.size(1) > D || table.size(1) % 2)
     Py_RETURN_NONE;
   const bool given = a[9] != Py_None;
@@ -513,7 +516,8 @@ PyObject *plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
 PyObject *tree(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   at::Tensor q, mask, out, ws, status_tensor;
-  if (n != 7 || !tensor(a[0], q) || !tensor(a[2], mask) || !q.is_cuda() || q.dim() != 4 || q.stride(3) != 1)
+  if (n != 7 || !tensor(a[0], q) || !tensor(a[2], mask) || !q.is_cuda() || q.dim() != 4 || q.stride(3) != 1 ||
+      q._fw_grad(0).defined())
     Py_RETURN_NONE;
   const int dtype = dtype_code(q.scalar_type());
   const int64_t B = q.size(0), Hq = q.size(1), Q = q.size(2), D = q.size(3);

@@ -269,6 +269,7 @@ def tree_decode_attention(q: torch.Tensor, kv: pa.PackedKV, mask: torch.Tensor, 
         got = _lib.host().tree(q, kv, mask, scale, out, workspace, status)
         if got is not None:
             return got
+    _lib.no_tangents("tree_decode_attention", q)
     pa.check_contract(q, kv, check_page_ids=check_page_ids)
     if not q.is_cuda:
         raise pa.UnsupportedLayout("the CUDA tree kernels need CUDA tensors")

@@ -5,7 +5,8 @@ cache's append and the attention (the reference leaves it to Transformers'
 modelling code): every head's row is normalised (optionally) and turned by its
 token's position, in fp32 with one rounding, straight from the projection's
 strided output into the tensors the next calls read (`wtq_qk_norm_rope`).
-Inference only, like the rest of the package: there is no backward pass.
+Inference only, like the rest of the package: there is no backward pass, and tensors that
+carry tangents are refused.
 """
 from __future__ import annotations
 
@@ -72,8 +73,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
         return got
     xs = [q, k] if v is None else [q, k, v]
     weights = [q_weight, k_weight]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*xs, *weights)):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*xs, *weights, table)):
         raise RuntimeError("qk_norm_rope has no backward pass: call it under torch.no_grad()")
+    _lib.no_tangents("qk_norm_rope", *xs, *weights, table)
     dev = _lib.require_cuda(*xs, positions, table, *(w for w in weights if w is not None))
     _lib.reachable("status", status)
     if any(t.dim() != 4 for t in xs) or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:] \
