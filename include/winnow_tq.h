@@ -343,10 +343,13 @@ int wtq_release_tokens(const int32_t *marks, int32_t *table, int64_t table_strid
  * whose bit is set in their mask.  q, out: element (b, head, token, d) at b * strides[0] + head *
  * strides[1] + token * strides[2] + d.  mask (B, Q, ceil(Q / 32)) int32 words, element strides {batch,
  * token}; a token whose words are all zero is padding and gets zeros.  A sequence shorter than Q has no
- * history, and tree tokens before its position 0 do not exist.  fp32 queries are computed in fp32 on the
- * CUDA cores; 16-bit queries on the tensor cores (fp16 operands, fp32 sums) where head_dim is 64 or 128,
- * the widths 4/4, 4/6, 6/6 or 8/8, the page size a power of two >= 16 and the pages 16-byte aligned,
- * otherwise in fp32 as well.  head_dim <= 256, B Q <= 2^24, B Q Hq < 2^31, max_pages S <= 2^30.  A tree
+ * history, and tree tokens before its position 0 do not exist.  The pages are scanned in fp32 on the CUDA
+ * cores, with 16-bit queries on the tensor cores where head_dim is 64 or 128, the widths 4/4, 4/6, 6/6 or 8/8,
+ * the page size a power of two >= 16 and the pages 16-byte aligned: scores of operands split into two fp16
+ * parts (off by 2^-21 of |q| |k|), probabilities and, for bf16, values rounded to fp16, fp32 sums.  Queries
+ * and results are turned by Pi, any finite matrix, at head_dim 64 and 128 (Pi 16-byte aligned) as products of
+ * factors split in the same way, off by 2^-21 of the largest elements' product a term, otherwise in
+ * fp32.  head_dim <= 256, B Q <= 2^24, B Q Hq < 2^31, max_pages S <= 2^30.  A tree
  * token whose norms are not finite reaches the tokens that see it only.  Status bits as for wtq_decode.  The
  * workspace (wtq_tree_workspace_bytes, 256-byte aligned) needs no preparation. */
 size_t wtq_tree_workspace_bytes(int B, int Hq, int Hkv, int Q, int D);

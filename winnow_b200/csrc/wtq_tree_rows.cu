@@ -6,7 +6,7 @@
 // products summed in fp32, which leaves 2^-22 of the result as error, the class of an fp32 product
 // (16-bit queries have no low part: two products; neither do states that leave as bf16, whose rounding is
 // eight times that of the fp16 high part).  A row is scaled by a power of two to its largest
-// element first, and Pi by 2^8, so that low parts stay clear of fp16's subnormal range.  Pi is laid out
+// element first, and Pi to 2^8 times its own, so that any matrix fits and low parts stay clear of fp16's subnormal range.  Pi is laid out
 // as the operand once and serves both: read along its rows for the queries (K-major), across them for
 // the states (MN-major).  A thread per row quarter converts and stores.  Bound by the reads of rows and of
 // Pi from L2: 13 and 21 us from a cold cache at 16 384 rows, where the CUDA-core kernels of wtq_tree.cu
@@ -30,7 +30,7 @@ constexpr float kPiScale = 256.f;
 template <int D> struct Map {
   static constexpr uint32_t kGroup = (uint32_t)D * 16u;     // eight rows of an operand
   static constexpr uint32_t kScales = 1024;                 // a row's power of two
-  static constexpr uint32_t kBar = kScales + 4 * kRows, kSlot = kBar + 8, kPrefix = kSlot + 8;
+  static constexpr uint32_t kBar = kScales + 4 * kRows, kSlot = kBar + 8, kMostPi = kSlot + 8, kPrefix = kMostPi + 4 * (kThreads / 32);
   static constexpr uint32_t kA = 10240, kABytes = kRows / 8 * kGroup, kBBytes = D / 8 * kGroup;
   static constexpr uint32_t kB = kA + kABytes, kALow = kB + 2 * kBBytes;     // the rows' low parts, where there are any
   static constexpr uint32_t kBytes = kALow + kABytes;
@@ -93,35 +93,58 @@ __global__ void __launch_bounds__(kThreads, WIDE ? 1 : 2) product_kernel(Params 
   }
   constexpr int kPieces = D / 8;
   const float *Pi = JOIN ? p.v.Pi : p.k.Pi;
-  if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(M::kSlot), "r"((uint32_t)D)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  constexpr int kPi = D * kPieces / kThreads;              // pieces of Pi of a thread
+  float4 pi[kPi][2];
+  {
+    float most = 0.f;
+#pragma unroll
+    for (int k = 0; k < kPi; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float4 a = pi[k][h] = __ldg(reinterpret_cast<const float4 *>(Pi + 8 * (tid + k * kThreads)) + h);
+        most = fmaxf(fmaxf(most, fmaxf(fabsf(a.x), fabsf(a.y))), fmaxf(fabsf(a.z), fabsf(a.w)));
+      }
+    const uint32_t of_warp = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+    if (lane == 0) sts_float(M::kMostPi + 4u * warp, __uint_as_float(of_warp));
   }
+  auto take_columns = [&] {
+    if (warp == 0) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(M::kSlot), "r"((uint32_t)D)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+  };
+  if constexpr (!JOIN) take_columns();
   if (tid == 0) {
     mbar_init(M::kBar, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  if constexpr (!JOIN) {
-    // Only now that this block has its tensor memory: a block of the scan that took all of it first would
-    // wait for this kernel while this block waited for it.
-    __syncthreads();
-    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-  }
-#pragma unroll
-  for (int e = tid; e < D * kPieces; e += kThreads) {
-    const int row = e / kPieces, piece = e % kPieces;
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(Pi + row * D + 8 * piece));
-    const float4 b = __ldg(reinterpret_cast<const float4 *>(Pi + row * D + 8 * piece) + 1);
-    const float x[8] = {a.x * kPiScale, a.y * kPiScale, a.z * kPiScale, a.w * kPiScale,
-                        b.x * kPiScale, b.y * kPiScale, b.z * kPiScale, b.w * kPiScale};
-    store_split(M::kB + (uint32_t)(row >> 3) * M::kGroup + (uint32_t)piece * 128u + (uint32_t)(row & 7) * 16u, M::kBBytes, x);
-  }
   int *prefix = reinterpret_cast<int *>(dyn_smem + (M::kPrefix - base));
   long long share = 1;
   if constexpr (JOIN) {
-    tile_prefix(p, prefix);
+    tile_prefix(p, prefix);                                 // (ends with a block barrier)
+  } else {
+    __syncthreads();
+    // Only now that this block has its tensor memory: a block of the scan that took all of it first would
+    // wait for this kernel while this block waited for it.
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  }
+  float most_pi = 0.f, inverse_pi;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) most_pi = fmaxf(most_pi, lds_float(M::kMostPi + 4u * w));
+  const float power_pi = power_of(most_pi, inverse_pi);
+#pragma unroll
+  for (int k = 0; k < kPi; ++k) {
+    const int row = (tid + k * kThreads) / kPieces, piece = (tid + k * kThreads) % kPieces;
+    const float4 a = pi[k][0], b = pi[k][1];
+    float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = x[e] * inverse_pi * kPiScale;
+    store_split(M::kB + (uint32_t)(row >> 3) * M::kGroup + (uint32_t)piece * 128u + (uint32_t)(row & 7) * 16u, M::kBBytes, x);
+  }
+  if constexpr (JOIN) {
     share = run_length(p, prefix);
+    take_columns();                                         // (which the scan's blocks give back at their end)
     asm volatile("griddepcontrol.wait;\n" ::: "memory");   // the states
   }
   // ---- the rows: kPieces lanes a row, several rows of a warp at a time ------------------------------
@@ -321,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, WIDE ? 1 : 2) product_kernel(Params 
     tmem_wait_load();
     if (row >= rows || !done) continue;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f * power_pi);
     if constexpr (!JOIN) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)

@@ -261,8 +261,10 @@ def tree_decode_attention(q: torch.Tensor, kv: pa.PackedKV, mask: torch.Tensor, 
     the history before them and the tree tokens whose bit is set in its words of `mask`, int32
     (B, Q, ceil(Q / 32)): bit j % 32 of word j // 32 (`plan_tokens` builds them from parents).  A token
     without any bit is padding and gets zeros.  Any number of query heads per kv head, any width and
-    page size, head_dim up to 256.  fp32 queries are computed in fp32; 16-bit ones on the tensor cores
-    where the layout allows (`wtq_tree_on_tensor_cores`), and in fp32 elsewhere.  `workspace`: uint8, at
+    page size, head_dim up to 256.  fp32 queries are scanned in fp32; 16-bit ones on the tensor cores
+    where the layout allows (`wtq_tree_on_tensor_cores`), with scores of split operands (off by 2^-21 of |q| |k|), and in
+    fp32 elsewhere.  At head_dim 64 and 128 both products with the rotations are split products of that
+    class for every dtype.  `workspace`: uint8, at
     least `tree_workspace_bytes`, 256-byte aligned, needs no preparation; calls that may overlap need
     one each."""
     if not check_page_ids:                     # checked, allocated for and launched in native code
