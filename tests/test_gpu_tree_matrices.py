@@ -36,3 +36,12 @@ def test_a_few_large_elements():
     for quant in (kv.k_quant, kv.v_quant):
         quant.Pi[3, 5] = 1000.0
     check(kv, 2, 8, 6, torch.float32, mult=1e-3)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,Hq,Q", [(1, 1, 1), (1, 3, 5), (2, 6, 21), (3, 14, 19)])
+def test_rows_that_leave_part_of_a_block_empty(B, Hq, Q, D):
+    """Blocks of 16 to 128 rows: lanes past the last one load with the others and store nothing."""
+    kv = build([90] * B, 1, D, 16, 4, 4)
+    for dtype in (torch.float32, torch.float16):
+        check(kv, B, Hq, Q, dtype)

@@ -340,6 +340,7 @@ __global__ void __launch_bounds__(kThreads, WIDE ? 1 : 2) product_kernel(Params 
 #pragma unroll 1
   for (int c0 = (warp >> 2) * (D / 4); c0 < ((warp >> 2) + 1) * (D / 4); c0 += 16) {
     uint32_t o[16];
+    __syncwarp();                                           // (lanes without a row are back from the last columns)
     tmem_load16(tmem + lanes + c0, o);
     tmem_wait_load();
     if (row >= rows || !done) continue;
