@@ -568,6 +568,7 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D, VLOW>::kThreads, 1) scan_kern
           l[2 * k + 1] = pack_half2(y.z - bf.x, y.w - bf.y);
         }
         const uint32_t to = tmem + lanes + (uint32_t)(kPart / 2 * st);
+        __syncwarp();                                       // (rows with and without queries: all issue what follows together)
         if constexpr (D == 128) {
           tmem_store32(to + kColQ, v);
           tmem_store32(to + kColQLow, l);
@@ -646,6 +647,7 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D, VLOW>::kThreads, 1) scan_kern
         }
         const float2 both = halves(add2(sums[0], sums[1]));
         sum += both.x + both.y;
+        __syncwarp();
         tmem_store32(s_addr, pr);                           // over the scores just read
         tmem_wait_store();
         fence_before();
@@ -685,6 +687,7 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D, VLOW>::kThreads, 1) scan_kern
 #pragma unroll 1
         for (int c0 = st * (D / 2); c0 < (st + 1) * (D / 2); c0 += 32) {
           uint32_t o[32], o1[32];
+          __syncwarp();                                     // (rows that store nothing are back from the last columns)
           tmem_load32<0>(tmem + lanes + kColO + c0, o);
           if (nt > 1) tmem_load32<0>(tmem + lanes + kColO + 128 + c0, o1);
           tmem_wait_load();
