@@ -377,8 +377,12 @@ __global__ void __launch_bounds__(kThreads, WIDE ? 1 : 2) product_kernel(Params 
   }
   fence_before();
   __syncthreads();
-  if (warp == 0)
+  if (warp == 0) {
+    // (after a wait that ran out the products end before their tensor memory goes to somebody else; bounded as well)
+    for (int spin = 0; spin < kWaitTries && !done; ++spin) done = mbar_try(M::kBar, 0u);
+    __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"((uint32_t)D) : "memory");
+  }
 }
 
 template <bool JOIN, int D, bool WIDE> int launch_blocks(const Params &p, int rows_per, int blocks, cudaStream_t stream) {
