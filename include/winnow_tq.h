@@ -350,8 +350,9 @@ int wtq_release_tokens(const int32_t *marks, int32_t *table, int64_t table_strid
  * and results are turned by Pi, any finite matrix, at head_dim 64 and 128 (Pi 16-byte aligned) as products of
  * factors split in the same way, off by 2^-21 of the largest elements' product a term, otherwise in
  * fp32.  head_dim <= 256, B Q <= 2^24, B Q Hq < 2^31, max_pages S <= 2^30.  A tree
- * token whose norms are not finite reaches the tokens that see it only.  Status bits as for wtq_decode.  The
- * workspace (wtq_tree_workspace_bytes, 256-byte aligned) needs no preparation. */
+ * token whose norms are not finite reaches the tokens that see it only.  A sequence longer than
+ * its table keeps its tree's place, without the tokens past the table (WTQ_STATUS_BAD_POSITION).  Status bits
+ * as for wtq_decode.  The workspace (wtq_tree_workspace_bytes, 256-byte aligned) needs no preparation. */
 size_t wtq_tree_workspace_bytes(int B, int Hq, int Hkv, int Q, int D);
 int wtq_tree(const void *q, int dtype, const int64_t q_strides[3], void *out, const int64_t out_strides[3],
              const wtq_side_t *k_side, const wtq_side_t *v_side, const int32_t *page_table,

@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(Params p) {
   for (long long x = begin; x < end;) {
     const Piece c = piece_at(p, prefix, x, begin, end);
     x += c.last - c.first;
-    const int L = length_of(p, c.b), hist = L - p.Q, row0 = c.rb * p.rows;
+    const int L = length_of(p, c.b), hist = history_of(p, c.b), places = places_of(p, c.b), row0 = c.rb * p.rows;
     const int32_t *table = p.page_table + (int64_t)c.b * p.table_stride;
     __syncthreads();
     {
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_kernel(Params p) {
         float w = 0.f, f = 1.f;
         if (!dead[k]) {
           const int32_t *words = p.mask + c.b * p.mask_b + (row0 + r) / p.n_rep * p.mask_t;
-          const uint32_t seen = visible(words, p.Q, tok0 - hist);
+          const uint32_t seen = visible(words, places, tok0 - hist);
           const float v = (seen >> lane & 1u) != 0 && tok0 + lane < L ? ps[r * kP + lane] : -INFINITY;
           const float now = fmaxf(m[k], warp_max(v));
           if ((now == -INFINITY && __any_sync(0xffffffffu, v != v)) || (seen & bad) != 0u) l[k] = NAN;

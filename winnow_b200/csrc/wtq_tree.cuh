@@ -42,15 +42,20 @@ __device__ __forceinline__ int length_of(const Params &p, int b) {
   const int L = p.seq_lens[b];
   return L < 0 ? 0 : L > p.max_tokens ? p.max_tokens : L;
 }
+// Tokens before a sequence's tree.  Its length as it is says where the tree stands, also where the table has no room
+// for all of it: tokens past the table do not exist then.
+__device__ __forceinline__ int history_of(const Params &p, int b) { return p.seq_lens[b] - p.Q; }
 __device__ __forceinline__ int tiles_of(const Params &p, int b) { return (length_of(p, b) + p.tile - 1) / p.tile; }
 
-// Exclusive prefix (B + 1 entries) of the sequences' tiles, by the whole block.
+// Exclusive prefix (B + 1 entries) of the sequences' tiles, by the whole block.  Lengths past the table are reported.
 __device__ __forceinline__ void tile_prefix(const Params &p, int *prefix) {
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
     int running = 0;
     for (int b0 = 0; b0 < p.B; b0 += 32) {
       const int n = b0 + lane < p.B ? tiles_of(p, b0 + lane) : 0;
+      if (blockIdx.x == 0 && b0 + lane < p.B && p.seq_lens[b0 + lane] > p.max_tokens && p.status)
+        atomicOr(p.status, WTQ_STATUS_BAD_POSITION);
       int incl = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -100,16 +105,20 @@ __device__ __forceinline__ Piece piece_at(const Params &p, const int *prefix, lo
   return c;
 }
 
+// Tree places of a sequence that the table has room for (negative: not even all of the history).
+__device__ __forceinline__ int places_of(const Params &p, int b) {
+  const int room = p.max_tokens - history_of(p, b);
+  return room < p.Q ? room : p.Q;
+}
 // 32 tokens from tree place `j0` on as bits, of a row with the mask words at `words`: places before
-// the tree are its history, places past it do not exist.
-__device__ __forceinline__ uint32_t visible(const int32_t *words, int Q, int j0) {
-  if (j0 <= -32) return 0xffffffffu;
+// the tree are its history, those from `places` on do not exist.
+__device__ __forceinline__ uint32_t visible(const int32_t *words, int places, int j0) {
+  if (j0 <= -32 && places >= 0) return 0xffffffffu;
   const int k = j0 >> 5, r = j0 & 31;     // (floor)
   auto word = [&](int i) -> uint32_t {
-    if (i < 0) return 0xffffffffu;
-    if (32 * i >= Q) return 0u;
-    const uint32_t w = (uint32_t)__ldg(words + i);
-    return Q - 32 * i >= 32 ? w : w & ((1u << (Q - 32 * i)) - 1u);
+    if (32 * i >= places) return 0u;
+    const uint32_t w = i < 0 ? 0xffffffffu : (uint32_t)__ldg(words + i);
+    return places - 32 * i >= 32 ? w : w & ((1u << (places - 32 * i)) - 1u);
   };
   return __funnelshift_r(word(k), word(k + 1), r);
 }

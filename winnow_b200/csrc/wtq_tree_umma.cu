@@ -383,7 +383,8 @@ __device__ __forceinline__ const int32_t *words_of(const Params &p, const Piece 
 // Bits of the 64 tokens from `tok0` on that query row `qr` sees.
 __device__ __noinline__ uint2 seen_tokens(const Params &p, int b, int qr, int at) {
   const int32_t *words = p.mask + b * p.mask_b + (int64_t)(qr / p.n_rep) * p.mask_t;
-  return make_uint2(visible(words, p.Q, at), visible(words, p.Q, at + 32));
+  const int places = places_of(p, b);
+  return make_uint2(visible(words, places, at), visible(words, places, at + 32));
 }
 
 // fp32 scores of query row `qr` (negative: zeros) with the 64 tokens from `tok0` on, from the packed codes,
@@ -394,7 +395,7 @@ __device__ __noinline__ void precise_scores(const Params &p, Piece c, int qr, in
   constexpr int kRowBytes = D * BW / 8;
   const int end = length_of(p, c.b), i = qr / p.n_rep;
   uint2 seen = make_uint2(kFull, kFull);
-  if (masked && qr >= 0) seen = seen_tokens(p, c.b, qr, tok0 - (end - p.Q));
+  if (masked && qr >= 0) seen = seen_tokens(p, c.b, qr, tok0 - history_of(p, c.b));
   const float *q = qr < 0 ? nullptr : p.q_rot + (((int64_t)c.b * p.Q + i) * p.Hq + c.h * p.n_rep + qr - i * p.n_rep) * D;
 #pragma unroll 1
   for (int blk = 0; blk < kTile / 16; ++blk) {                 // sixteen tokens of one page
@@ -434,7 +435,7 @@ __device__ __noinline__ void precise_scores(const Params &p, Piece c, int qr, in
 
 // Whether query row `qr` (negative: none) sees a token of the piece whose value norm is not finite.
 __device__ __noinline__ bool spoiled(const Params &p, Piece c, int qr) {
-  const int L = length_of(p, c.b), hist = L - p.Q, lane = threadIdx.x & 31;
+  const int L = length_of(p, c.b), hist = history_of(p, c.b), places = places_of(p, c.b), lane = threadIdx.x & 31;
   const int32_t *words = p.mask + c.b * p.mask_b + (int64_t)(max(qr, 0) / p.n_rep) * p.mask_t;
   bool found = false;
   for (int tok0 = c.first * kTile; tok0 < min(L, c.last * kTile); tok0 += 32) {
@@ -446,7 +447,7 @@ __device__ __noinline__ bool spoiled(const Params &p, Piece c, int qr) {
       bad = !(fabsf(n) < INFINITY);
     }
     const uint32_t all = __ballot_sync(kFull, bad);
-    if (all != 0u && qr >= 0) found = found || (visible(words, p.Q, tok0 - hist) & all) != 0u;
+    if (all != 0u && qr >= 0) found = found || (visible(words, places, tok0 - hist) & all) != 0u;
   }
   return found;
 }
@@ -545,7 +546,7 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D, VLOW>::kThreads, 1) scan_kern
       const Piece c = piece_at(p, prefix, x, begin, end);
       const int nt = c.last - c.first;
       x += nt;
-      const int L = length_of(p, c.b), hist = L - p.Q, qr = c.rb * kRows + r;
+      const int hist = history_of(p, c.b), all_see = min(hist, p.max_tokens), qr = c.rb * kRows + r;
       const bool live = qr < p.R && !padding(words_of(p, c, qr), p.Q);
       const bool working = __any_sync(kFull, live);         // a warp without live rows only keeps step
       auto row_of = [&]() -> int64_t {                      // of the (B, Q, Hq) states
@@ -595,7 +596,7 @@ __global__ void __launch_bounds__(Map<BWK, BWV, D, VLOW>::kThreads, 1) scan_kern
         tmem_load32<0>(s_addr, s);
         tmem_load32<32>(s_addr + 32, s);
         tmem_wait_load();
-        const bool masked = tok0 + kTile > hist;
+        const bool masked = tok0 + kTile > all_see;
         bool sees = live;
         if (masked) {
           uint2 seen = make_uint2(kFull, kFull);
