@@ -128,6 +128,7 @@ class DevicePages:
         if pool.held(owner):
             raise ValueError(f"{owner!r} already holds pages")
         ids = [ref.page for ref in pool.ensure(owner, pages * pool.page_size)]
+        self._reservation = pool.reservation(owner)
         dev = pool.device
         self.free_pages = torch.tensor(ids[::-1], dtype=torch.int32, device=dev)
         self.free_count = torch.tensor([len(ids)], dtype=torch.int32, device=dev)
@@ -138,10 +139,17 @@ class DevicePages:
         self._ticket = torch.zeros(1, dtype=torch.int32, device=dev)
         self._room: dict = {}
 
+    def ensure_held(self) -> None:
+        """Raise `StalePage` once the pages have been given back (`close`, or a release of the owner in the pool):
+        they may be another request's by then."""
+        if self.pool.reservation(self.owner) is not self._reservation:
+            raise StalePage(f"{self.owner!r} no longer holds the pages of this batch")
+
     def extend(self, new_tokens=None, *, tokens: int | None = None, parents=None) -> TokenPlan:
         """Append new_tokens[b] tokens (`tokens` in all, or room for more), or a tree each.  The plan's
         per-token tensors are this object's own and written again by a later call for about as many
         tokens; its state tensors are `lengths`, `held`, `free_count`."""
+        self.ensure_held()
         B = self.lengths.numel()
         if parents is not None:
             Q = int(parents.shape[1]) if parents.dim() == 2 else 0
@@ -172,6 +180,7 @@ class DevicePages:
         pool = self.pool
         if pool.dense:
             raise ValueError("keep serves packed pools")
+        self.ensure_held()
         after = keep_tokens(pool.k_pages, pool.k_norms, pool.v_pages, pool.v_norms, self.table, self.lengths, keep,
                             counts, drafted, granted=None if plan is None else plan.starts[-1:], status=self.status)
         self.lengths.copy_(after)
@@ -179,6 +188,7 @@ class DevicePages:
 
     def release(self, marks: torch.Tensor) -> None:
         """End the sequences with marks[b] != 0: their pages are free for the next `extend`."""
+        self.ensure_held()
         dev = _lib.require_cuda(marks, self.table)
         _int32("marks", marks, self.lengths.numel())
         with torch.cuda.device(dev):
@@ -201,5 +211,7 @@ class DevicePages:
                         f"{_lib.STATUS_BAD_PARENT} parent behind its child)")
 
     def close(self, fence=None) -> int:
-        """Give all pages back to the pool, behind a fence."""
+        """Give all pages back to the pool, behind a fence; calls that would use them after that raise `StalePage`."""
+        if self.pool.reservation(self.owner) is not self._reservation:
+            return 0                                       # (given back already; the name may be another's)
         return self.pool.release(self.owner, fence)

@@ -199,6 +199,7 @@ class TreeSession:
         projection when the session has a `rotary`."""
         if self.plan is None:
             raise RuntimeError("begin() comes before layer()")
+        self.pages.ensure_held()
         kv, status = self._layers[layer_idx], self.pages.status
         if self.rotary is not None:
             positions = self.plan.positions.view(-1, self.drafted)

@@ -215,6 +215,10 @@ class PagePool:
             self._sweep()
             return len(res.pages)
 
+    def reservation(self, owner: str):
+        """What `owner` holds, as an object that is its own until the next `release`; None if nothing."""
+        return self._held.get(owner)
+
     def reclaim(self) -> int:
         with self._lock:
             return self._sweep()
