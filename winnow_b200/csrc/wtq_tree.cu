@@ -135,7 +135,8 @@ __global__ void __launch_bounds__(kRowThreads) join_kernel(Params p) {
 // shared memory four coordinates at a time (6 loads for 32 products).  Softmax: a warp has 8 rows, a
 // lane per token.  Values: a thread has 4 rows x 4 NJ coordinates (NJ + 1 loads for 16 NJ products a
 // token).  Bound by shared-memory operands at long histories, by latency at short ones: a call of 8
-// tokens over 1000, 8 heads on 2, takes 45 us with both products.
+// tokens over 1000, 8 heads on 2, takes 49 us with both products; 16 x 8192 tokens, 128 rows a kv head,
+// 4.2 ms (16.5 TFLOP/s).
 constexpr int kScanThreads = 256, kScanRows = 64, kScanTile = 32;
 
 __host__ __device__ inline int scan_pitch(int D) { return (D + 3) / 4 * 4 + 4; }

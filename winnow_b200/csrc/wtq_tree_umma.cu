@@ -9,8 +9,8 @@
 //   fetch     a warp per side: codes and norms of a tile into a ring of raw tiles, 16 bytes a copy;
 //   decode    eight warps per side, one for every 8 tokens of a tile (four for 4-bit values without low parts):
 //             codes through the per-lane lookup tables to centroid times norm as fp16 high and low parts in the
-//             canonical operand layout, as many tiles deep as shared memory has room for (two or three; 8 bits at
-//             head_dim 128: one);
+//             canonical operand layout, as many tiles deep as shared memory has room for (two or three; one of the
+//             values for fp16 results at head_dim 128, but for 6 bits);
 //   multiply  a warp for S = Qlow Khigh + Qhigh Klow + Qhigh Khigh (N 64) and one for O += P V (A = P from tensor
 //             memory, V read with tokens as the contraction), an elected lane of each issues;
 //   softmax   a warpgroup per stream, a thread per query row: scores from tensor memory, tree mask, running maximum,
@@ -31,11 +31,12 @@
 //
 // A warp on its own gets through an instruction in about nine cycles here, so a role is only as fast
 // as its instructions per tile are few and lie in the instruction cache, which is why sides of one width share theirs.
-// Bound by shared memory: lookups (8 bytes a pair of codes with low parts), operand stores and the products' reads of them
-// take two thirds of its cycles.  Queries' low parts in tensor memory, with the probabilities over the scores, and raw
-// rows turned against bank conflicts took 16 x 8 kv heads x 8192 tokens, 128 rows a group, 4 bits, bf16 from 215 to 167 us with
-// both rotations, and 8 x 131 072 tokens, 512 rows a group, fp16 from 820 to 560 us.  (Single products, without low parts
-// on either side: 145 and 400 us.)
+// Bound by shared memory: loads (lookups, 8 bytes a pair of codes with low parts) and operand stores take half of its
+// cycles, and the products, whose pipe is active 46 % of the time, read their operands through the rest.  Queries' low parts
+// in tensor memory, with the probabilities over the scores, and raw rows turned against bank conflicts took
+// 16 x 8 kv heads x 8192 tokens, 128 rows a group, 4 bits, bf16 from 215 to 171 us with both rotations, and
+// 8 x 131 072 tokens, 512 rows a group, fp16 from 820 to 560 us; now 173 (up to 194 where calls follow one another for
+// long) and 575 (676), 478 TFLOP/s.  (Single products, without low parts on either side: 145 and 400 us.)
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
