@@ -211,10 +211,12 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
     return dev
 
 
-def reachable(what: str, t: torch.Tensor | None) -> None:
-    """A buffer the kernels write beside their operands: device memory, or pinned host memory."""
+def reachable(what: str, t: torch.Tensor | None, device: torch.device | None = None) -> None:
+    """A buffer the kernels write beside their operands: device memory (of `device`, if given), or pinned host memory."""
     if t is not None and t.device.type == "cpu" and not t.is_pinned():
         raise BackendError(f"{what} is in pageable host memory, which the kernels cannot reach")
+    if t is not None and device is not None and t.is_cuda and t.device != device:
+        raise BackendError(f"{what} is on {t.device}, the operands on {device}")
 
 
 def no_tangents(what: str, *tensors: torch.Tensor | None) -> None:

@@ -63,8 +63,8 @@ def plan_tokens(lengths, new_tokens, table, held, free_pages, free_count, page_s
         if got is not None:
             return TokenPlan(*got)
     dev = _lib.require_cuda(lengths, table, held, free_pages, free_count, parents if tree else new_tokens)
-    _lib.reachable("status", status)
-    _lib.reachable("ticket", ticket)
+    _lib.reachable("status", status, dev)
+    _lib.reachable("ticket", ticket, dev)
     if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) != 1 or table.shape[1] < 1:
         raise ValueError("table must be int32 (B, width) with contiguous rows")
     B, W = table.shape

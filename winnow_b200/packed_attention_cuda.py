@@ -295,8 +295,10 @@ def tree_decode_attention(q: torch.Tensor, kv: pa.PackedKV, mask: torch.Tensor, 
         out = torch.empty(B, Q, Hq, D, dtype=q.dtype, device=dev).permute(0, 2, 1, 3)
     elif tuple(out.shape) != (B, Hq, Q, D) or out.dtype != q.dtype or out.device != dev or out.stride(-1) != 1:
         raise pa.UnsupportedLayout("out must be (B, Hq, Q, D) in q.dtype with unit stride in D")
-    _lib.reachable("workspace", workspace)
-    _lib.reachable("status", status)
+    _lib.reachable("workspace", workspace, dev)
+    _lib.reachable("status", status, dev)
+    if workspace is not None and not workspace.is_contiguous():
+        raise pa.UnsupportedLayout("the workspace must be contiguous")
     if B == 0 or Q == 0:
         return out
     Hkv, S, P = kv.num_kv_heads, kv.page_size, kv.k_pages.shape[0]

@@ -301,7 +301,7 @@ def keep_tokens(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, 
     if got is not None:
         return got
     dev = _lib.require_cuda(k_pages, k_norms, v_pages, v_norms, page_table, seq_lens, keep, counts)
-    _lib.reachable("status", status)
+    _lib.reachable("status", status, dev)
     if drafted < 0:
         raise ValueError("drafted must not be negative")
     if k_pages.dim() != 5 or v_pages.dim() != 5 or v_pages.shape[:4] != k_pages.shape[:4]:

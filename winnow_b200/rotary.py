@@ -77,7 +77,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
         raise RuntimeError("qk_norm_rope has no backward pass: call it under torch.no_grad()")
     _lib.no_tangents("qk_norm_rope", *xs, *weights, table)
     dev = _lib.require_cuda(*xs, positions, table, *(w for w in weights if w is not None))
-    _lib.reachable("status", status)
+    _lib.reachable("status", status, dev)
     if any(t.dim() != 4 for t in xs) or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:] \
             or (v is not None and v.shape != k.shape):
         raise ValueError("q must be (B, Hq, n, D), k and v (B, Hkv, n, D)")
