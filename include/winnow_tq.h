@@ -323,7 +323,7 @@ int wtq_qk_norm_rope(const wtq_rope_side_t sides[3], int dtype, int weight_dtype
  * masks are 0, and WTQ_STATUS_NO_PAGES is set (WTQ_STATUS_BAD_POSITION for negative numbers or more new
  * tokens than `tokens`).  State outputs may be the inputs that they advance; then `ticket`, a device word that is
  * zero between calls, must be given.  Otherwise outputs and the table share memory neither with inputs nor with one
- * another.  B <= 4096. */
+ * another.  B <= 4096, tokens and stack <= 2^30. */
 typedef struct {
   int32_t *seq_lens, *held, *free_count, *starts, *sequence, *positions, *slot_pages, *slot_ends, *mask;
 } wtq_plan_t;

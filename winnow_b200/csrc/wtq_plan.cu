@@ -19,6 +19,7 @@ namespace plan {
 
 constexpr int kThreads = 256;
 constexpr int kMaxBatch = 4096;                 // two prefixes of it in shared memory
+constexpr int kMost = 1 << 30;                  // tokens and pages: a grid's stride past them is still an int
 
 struct Params {
   const int32_t *lengths, *new_tokens, *parents;
@@ -255,6 +256,8 @@ extern "C" int wtq_plan_tokens(const int32_t *lengths, const int32_t *new_tokens
                                int32_t *status, void *stream_) {
   if (B < 0 || B > plan::kMaxBatch || max_pages < 1 || S < 1 || tokens < 0 || drafted < 0 || stack < 0)
     return fail(WTQ_ERR_ARG, "wtq_plan_tokens: need 0 <= B <= %d and sizes that are not negative", plan::kMaxBatch);
+  if (tokens > plan::kMost || stack > plan::kMost)
+    return fail(WTQ_ERR_ARG, "wtq_plan_tokens: tokens and free pages are limited to 2^30");
   if (!out) return fail(WTQ_ERR_ARG, "wtq_plan_tokens: null outputs");
   if (parents ? drafted < 1 || (int64_t)B * drafted != tokens : drafted != 0)
     return fail(WTQ_ERR_ARG, "wtq_plan_tokens: with parents there are B * drafted tokens, without none is drafted");
@@ -298,6 +301,7 @@ extern "C" int wtq_release_tokens(const int32_t *marks, int32_t *table, int64_t 
                                   int stack, int32_t *status, void *stream_) {
   if (B < 0 || B > plan::kMaxBatch || max_pages < 1 || stack < 0)
     return fail(WTQ_ERR_ARG, "wtq_release_tokens: need 0 <= B <= %d", plan::kMaxBatch);
+  if (stack > plan::kMost) return fail(WTQ_ERR_ARG, "wtq_release_tokens: free pages are limited to 2^30");
   if (B == 0) return WTQ_OK;
   if (!marks || !table || !lengths || !held || !free_pages || !free_count)
     return fail(WTQ_ERR_ARG, "wtq_release_tokens: null argument");
